@@ -105,7 +105,12 @@ def draw(rng):
     c["L"] = {"decode": 1, "verify": rng.randint(2, 8), "prefill": _log_int(rng, 9, 1024)}[mode]
     if mode == "prefill" and rng.random() < 0.3:
         c["window"] = rng.choice([128, 512, 1024])
-    most = min(131072, MOST_CACHE // (c["B"] * hkv * (d + dv)), MOST_PAIRS // (c["B"] * hq * c["L"] * (d + dv)))
+    # a query sees L tokens at least
+    c["L"] = min(c["L"], math.isqrt(MOST_PAIRS // (c["B"] * hq * (d + dv))))
+    # 8-bit codes and small groups take more bytes an element than the listed 4-bit cache's groups of 64
+    bits = (d * kb + dv * vb) / (d + dv) + 32 / group
+    most = min(131072, int(MOST_CACHE * 4.5 / bits) // (c["B"] * hkv * (d + dv)),
+               MOST_PAIRS // (c["B"] * hq * c["L"] * (d + dv)))
     c["tokens"] = max(c["L"], _log_int(rng, 16, max(17, most)))
     if mode != "prefill" and c["B"] > 1 and rng.random() < 0.5:
         c["shortest"] = max(c["L"], int(c["tokens"] * rng.uniform(0.1, 1.0)))
