@@ -133,7 +133,7 @@ def _lengths(case):
 
 
 def _axis_of(case):
-    """The axis that each frequency's position comes from: contiguous sections, the first axis has the rest."""
+    """The axis that each frequency's position comes from: contiguous sections, the last axis has the rest."""
     n, a = case["rot"] // 2, case["axes"]
     part = n // a
     return [min(i // part, a - 1) if a > 1 else 0 for i in range(n)]
