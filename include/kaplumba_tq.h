@@ -356,6 +356,92 @@ int tq_attention_noalloc(const void* q, int q_dtype, int B, int Hq, int Hkv, int
                          int64_t capacity, int64_t max_tokens, const int32_t* seq_starts,
                          const int32_t* seq_lens, int causal, void* out, void* stream);
 
+/*
+ * Norms of the queries and keys of each head and the rotation by their
+ * positions, in one launch: for every vector x of q and k,
+ *   y   = x / sqrt(mean(x^2) + eps) * w      (y = x on a side without weight)
+ *   a_i = position(axis_i) * inv_freq[i]     i = 0 .. rot_dim / 2 - 1
+ *   (y_j, y_k) -> factor * (y_j cos a_i - y_k sin a_i, y_j sin a_i + y_k cos a_i)
+ * with (j, k) = (i, i + rot_dim / 2), or (2 i, 2 i + 1) when adjacent != 0;
+ * coordinates from rot_dim on are not turned.  Everything is computed in f32
+ * (angles in 64 bits) and rounded once.  What a layer does to its queries and
+ * keys before the append (llama.py:90-91 of the reference, which has the
+ * rotation alone).
+ * q, k: [B, H, L, dim] with element strides, last dim contiguous; outputs
+ * contiguous [B, H, L, dim] in the same dtype, which may not overlap the inputs.
+ * Either side may have no heads.  dim: 2..512; rot_dim: even, 0..dim (0: no
+ * rotation).  Weights: dim values of weight_dtype, each may be NULL.
+ * positions: NULL (token l is at start + l) or device integers of
+ * position_bytes 4 or 8 with element strides (axis, b, l); axis: device int32
+ * of rot_dim / 2 values in [0, axes) (others count as the nearest), NULL with
+ * one axis.
+ */
+int tq_norm_rope(const void* q, const void* k, int dtype, int B, int Hq, int Hk, int L, int dim,
+                 int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, int64_t k_stride_b,
+                 int64_t k_stride_h, int64_t k_stride_l, const void* q_weight,
+                 const void* k_weight, int weight_dtype, float eps, int rot_dim, int adjacent,
+                 const float* inv_freq, float factor, const int32_t* axis, int axes,
+                 const void* positions, int position_bytes, int64_t start, int64_t pos_stride_a,
+                 int64_t pos_stride_b, int64_t pos_stride_l, void* q_out, void* k_out,
+                 void* stream);
+
+/*
+ * Append L tokens of keys and values to a group-affine cache, in one launch.
+ * For every group of `group` (32, 64 or 128) coordinates of a vector, with
+ * n = 2^bits - 1 (bits 4 or 8, per side):
+ *   lo, hi = least and greatest value;  bias = lo
+ *   scale  = (hi - lo) / n in f32, rounded to dtype (0 below 2^-100)
+ *   code_i = number of half steps (k + 1/2) * scale, k = 0 .. n - 1, that
+ *            x_i - lo (in f32) reaches
+ * A group with an infinity or NaN gets NaN for scale and bias.  Counterpart of
+ * the reference's affine caches (MixedQuantKVCache, mixed_quant_cache.py: 8-bit
+ * keys, 4-bit values); codes are its packed rows, the pairs are stored side by
+ * side.
+ *   codes  : [B, H, capacity, dim * bits / 32] uint32, coordinate i at bits i * bits
+ *   params : [B, H, capacity, dim / group, 2] (scale, bias) in dtype
+ * dims: multiples of group, to 512; x and its strides 16-byte aligned.
+ */
+int tq_append_affine_kv(const void* k, const void* v, int dtype, int B, int H, int L, int k_dim,
+                        int v_dim, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_l,
+                        int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_l, int k_bits,
+                        int v_bits, int group, uint32_t* k_codes, void* k_params,
+                        uint32_t* v_codes, void* v_params, int64_t capacity, int64_t offset,
+                        void* stream);
+
+/*
+ * scale * code + bias of T tokens per (batch, head), in f32, stored as
+ * out_dtype [B, H, T, dim]: the first T rows of every [capacity] row block
+ * that codes and params point into.
+ */
+int tq_dequantize_affine(const uint32_t* codes, const void* params, int dtype, int B, int H, int T,
+                         int dim, int bits, int group, int64_t capacity, void* out, int out_dtype,
+                         void* stream);
+
+/*
+ * Attention straight from the group-affine cache:
+ *   s_t = scale * <q, k_t>,  k_t = scale_k code_k + bias_k
+ *   o   = sum_t p_t v_t / sum_t p_t,  p = softmax(s)
+ * q is [B, Hq, L, k_dim] in q_dtype, which is also the dtype of the params; out
+ * is contiguous [B, Hq, L, v_dim].  Scores, weights and sums are in f32 or
+ * more (the scale is not rounded to q_dtype).  seq_starts, seq_lens, causal and
+ * the mask follow tq_attention_general: masked scores are -FLT_MAX, a row that
+ * sees no key weighs all its tokens alike, a row whose every score is -inf and
+ * a sequence without tokens give zeros.  What a mask leaves out may hold NaN.
+ * Dims as in tq_append_affine_kv.  Workspace: at least
+ * tq_attention_affine_workspace_size() bytes, 256-byte aligned, no initial
+ * contents; it grows with B, L and max_tokens.
+ */
+int64_t tq_attention_affine_workspace_size(int B, int Hq, int Hkv, int L, int k_dim, int v_dim,
+                                           int64_t max_tokens);
+int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int L, int k_dim,
+                        int v_dim, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l,
+                        float scale, const uint32_t* k_codes, const void* k_params, int k_bits,
+                        const uint32_t* v_codes, const void* v_params, int v_bits, int group,
+                        int64_t capacity, int64_t max_tokens, const int32_t* seq_starts,
+                        const int32_t* seq_lens, int causal, const void* mask, int mask_kind,
+                        const int64_t* mask_strides, void* out, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,6 +114,31 @@ SIGNATURES = {
         c_int, c_int64, c_int64, c_void_p, c_void_p, c_int,    # norm dtype, cap, T, starts, lens, causal
         c_void_p, c_int, c_void_p,                             # mask, mask_kind, mask_strides (5 x int64)
         c_void_p, c_void_p, c_int64, c_void_p]),               # out, workspace, ws bytes, stream
+    "tq_norm_rope": (c_int, [
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,  # q, k, dtype, B, Hq, Hk, L, dim
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,  # q strides, k strides
+        c_void_p, c_void_p, c_int, c_float,                    # q weight, k weight, weight dtype, eps
+        c_int, c_int, c_void_p, c_float, c_void_p, c_int,      # rot_dim, adjacent, inv_freq, factor, axis, axes
+        c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,   # positions, their bytes, start, strides (axis, b, l)
+        c_void_p, c_void_p, c_void_p]),                        # q out, k out, stream
+    "tq_append_affine_kv": (c_int, [
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,  # k, v, dtype, B, H, L, k_dim, v_dim
+        c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,  # k strides, v strides
+        c_int, c_int, c_int,                                   # k_bits, v_bits, group
+        c_void_p, c_void_p, c_void_p, c_void_p,                # k codes, k params, v codes, v params
+        c_int64, c_int64, c_void_p]),                          # capacity, offset, stream
+    "tq_dequantize_affine": (c_int, [
+        c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,  # codes, params, dtype, B, H, T, dim, bits, group
+        c_int64, c_void_p, c_int, c_void_p]),                  # capacity, out, out dtype, stream
+    "tq_attention_affine_workspace_size": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int,
+                                                     c_int64]),
+    "tq_attention_affine": (c_int, [
+        c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,  # q, dtype, B, Hq, Hkv, L, k_dim, v_dim
+        c_int64, c_int64, c_int64, c_float,                    # q strides, scale
+        c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int,  # k codes, params, bits, v codes, params, bits, group
+        c_int64, c_int64, c_void_p, c_void_p, c_int,           # cap, T, starts, lens, causal
+        c_void_p, c_int, c_void_p,                             # mask, mask_kind, mask_strides (5 x int64)
+        c_void_p, c_void_p, c_int64, c_void_p]),               # out, workspace, ws bytes, stream
 }
 
 # Scratch bytes up to which tq_attention_noalloc takes every problem (TQ_NOALLOC_SCRATCH_BYTES in the header).

@@ -11,6 +11,9 @@ Storage per TurboQuant layer (all in HBM, contiguous, capacity grows in
   keys.indices  (B, H_kv, cap, PW_k) uint32   LSB-first packed codebook indices
   keys.norms    (B, H_kv, cap)       f32 (default) or f16 (reference layout)
   values.*      the same with the value codec
+and per group-affine layer (``QuantizedKVCache``), likewise:
+  keys.codes    (B, H_kv, cap, Dk * bits / 32) uint32   LSB-first 4- or 8-bit codes
+  keys.params   (B, H_kv, cap, Dk / group_size, 2)      (scale, bias) in the model dtype
 """
 from __future__ import annotations
 
@@ -21,11 +24,14 @@ from typing import Any, Dict, List, NamedTuple, Optional, Sequence
 import torch
 
 from . import ops
+from .affine import (AffineState, _check_bits, _check_dim, _check_group, affine_state, append_affine_kv,
+                     attention_affine, dequantize_affine)
 from .codebook import DEFAULT_TURBOQUANT_SEED
 from .prod import ProdCodec, TurboQuantProdState, attention_prod
 
 __all__ = [
-    "TurboQuantMSEState", "TurboQuantProdState", "TurboQuantKVCache", "KVCache", "make_prompt_cache",
+    "TurboQuantMSEState", "TurboQuantProdState", "TurboQuantKVCache", "KVCache", "QuantizedKVCache",
+    "make_prompt_cache",
     "save_prompt_cache", "load_prompt_cache", "can_trim_prompt_cache", "trim_prompt_cache",
     "create_attention_mask", "create_causal_mask",
 ]
@@ -560,6 +566,13 @@ class KVCache(_BaseCache):
             tq.update_and_fetch(self.keys[..., : self.offset, :], self.values[..., : self.offset, :])
         return tq
 
+    def to_quantized(self, group_size: int = 64, bits: int = 4, **kw) -> "QuantizedKVCache":
+        """The same tokens in a group-affine cache."""
+        q = QuantizedKVCache(group_size=group_size, bits=bits, **kw)
+        if self.keys is not None and self.offset > 0:
+            q.update_and_fetch(self.keys[..., : self.offset, :], self.values[..., : self.offset, :])
+        return q
+
     def make_mask(self, *args, **kwargs):
         return create_attention_mask(*args, offset=self.offset, **kwargs)
 
@@ -571,6 +584,156 @@ class KVCache(_BaseCache):
         if self.keys is None:
             return 0
         return sum(t.numel() * t.element_size() for t in (self.keys, self.values))
+
+
+class QuantizedKVCache(_BaseCache):
+    """Group-affine cache: 4- or 8-bit codes with a scale and a bias per group.
+
+    ``bits`` for both sides, or ``key_bits`` / ``val_bits`` of their own (the
+    reference's mixed cache keeps 8-bit keys and 4-bit values,
+    mixed_quant_cache.py:15-206).  Head dims are multiples of ``group_size``
+    (32, 64 or 128) up to 512, and may differ between keys and values; the
+    model dtype (f32, f16 or bf16) is the first append's.
+    """
+
+    step = 256
+
+    def __init__(self, group_size: int = 64, bits: int = 8, *, key_bits: Optional[int] = None,
+                 val_bits: Optional[int] = None):
+        self.group_size = _check_group(group_size)
+        self.bits = _check_bits(bits)
+        self.key_bits = _check_bits(bits if key_bits is None else key_bits)
+        self.val_bits = _check_bits(bits if val_bits is None else val_bits)
+        self.offset = 0
+        self.keys: Optional[AffineState] = None
+        self.values: Optional[AffineState] = None
+
+    def _alloc(self, B: int, H: int, cap: int, k_dim: int, v_dim: int, dtype, device) -> None:
+        self.keys = affine_state(B, H, cap, k_dim, self.key_bits, self.group_size, dtype, device)
+        self.values = affine_state(B, H, cap, v_dim, self.val_bits, self.group_size, dtype, device)
+
+    def _grow(self, st: AffineState, needed: int) -> AffineState:
+        if st.codes.shape[2] >= needed:
+            return st
+        cap = (needed + self.step - 1) // self.step * self.step
+        grown = AffineState(*(t.new_zeros(t.shape[:2] + (cap,) + t.shape[3:]) for t in st))
+        if self.offset > 0:
+            for dst, src in zip(grown, st):
+                dst[:, :, : self.offset].copy_(src[:, :, : self.offset])
+        return grown
+
+    def reserve(self, n_tokens: int, batch: int, n_kv_heads: int, k_dim: int, v_dim: int, device,
+                dtype: torch.dtype = torch.bfloat16) -> None:
+        """Preallocate capacity for ``n_tokens`` (no regrowth)."""
+        if self.keys is None:
+            self._alloc(batch, n_kv_heads, n_tokens, k_dim, v_dim, dtype, device)
+        else:
+            self.keys, self.values = self._grow(self.keys, n_tokens), self._grow(self.values, n_tokens)
+
+    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
+        """Quantize and append (B, H, L, D) keys and values."""
+        ops._require_device(keys, values)
+        B, H, L = keys.shape[0], keys.shape[1], keys.shape[2]
+        end = self.offset + L
+        if self.keys is None:
+            for t, what in ((keys, "key"), (values, "value")):
+                _check_dim(t.shape[-1], self.group_size, what)
+            cap = (end + self.step - 1) // self.step * self.step
+            self._alloc(B, H, max(cap, self.step), keys.shape[-1], values.shape[-1], keys.dtype, keys.device)
+        else:
+            if self.keys.codes.shape[:2] != (B, H):
+                raise ValueError(f"batch/heads {(B, H)} differ from the cache's {tuple(self.keys.codes.shape[:2])}")
+            self.keys, self.values = self._grow(self.keys, end), self._grow(self.values, end)
+        append_affine_kv(keys, values, self.keys, self.values, self.offset, self.group_size)
+        self.offset = end
+        ks, vs = self.state
+        return (_QuantizedStateProxy(ks, end, H, keys.shape[-1], B),
+                _QuantizedStateProxy(vs, end, H, values.shape[-1], B))
+
+    def _states(self, keys_state, values_state):
+        if keys_state is None or values_state is None:
+            if self.keys is None:
+                raise ValueError("the cache holds no tokens yet")
+            keys_state, values_state = self.state
+        return _unwrap(keys_state), _unwrap(values_state)
+
+    def dequantize(self, keys_state=None, values_state=None, dtype: Optional[torch.dtype] = None):
+        """Keys and values (B, H, T, D) that the codes stand for, in the model dtype or ``dtype``."""
+        ks, vs = self._states(keys_state, values_state)
+        return (dequantize_affine(ks, self.group_size, dtype), dequantize_affine(vs, self.group_size, dtype))
+
+    def quantized_attention(self, queries, keys_state=None, values_state=None, scale: float = 1.0, mask=None):
+        """Attention of any number of queries straight from the codes."""
+        ks, vs = self._states(keys_state, values_state)
+        causal, arr = _split_mask(mask, queries.shape[-2])
+        return attention_affine(queries, ks, vs, self.group_size, scale, causal, mask=arr)
+
+    def decode_attention(self, queries, keys_state=None, values_state=None, scale: float = 1.0, mask=None):
+        if queries.shape[-2] != 1:
+            raise ValueError("decode attention expects a single query token.")
+        return self.quantized_attention(queries, keys_state, values_state, scale, mask)
+
+    def prefill_attention(self, queries, keys_state=None, values_state=None, scale: float = 1.0, mask=None):
+        return self.quantized_attention(queries, keys_state, values_state, scale, mask)
+
+    def size(self):
+        return self.offset
+
+    @property
+    def state(self):
+        """(key state, value state) of the tokens held."""
+        if self.keys is None:
+            return []
+        o = self.offset
+        return tuple(AffineState(st.codes[:, :, :o], st.params[:, :, :o]) for st in (self.keys, self.values))
+
+    @state.setter
+    def state(self, value):
+        if value is None or len(value) == 0:
+            self.keys, self.values = None, None
+            self.offset = 0
+            return
+        if len(value) != 2:
+            raise ValueError(f"Expected (key_state, val_state), got {len(value)} entries")
+        self.keys, self.values = (AffineState(*(t.contiguous() for t in st)) for st in value)
+        self.offset = self.keys.codes.shape[2]
+
+    @property
+    def meta_state(self):
+        """(offset, group_size, bits, key_bits, val_bits) as strings."""
+        return tuple(map(str, (self.offset, self.group_size, self.bits, self.key_bits, self.val_bits)))
+
+    @meta_state.setter
+    def meta_state(self, value):
+        if len(value) not in (3, 5):
+            raise ValueError(f"QuantizedKVCache meta_state has {len(value)} fields; expected 3 or 5")
+        offset, group, bits = (int(x) for x in value[:3])
+        kb, vb = (int(x) for x in value[3:5]) if len(value) == 5 else (bits, bits)
+        held = self.keys.codes.shape[2] if self.keys is not None else 0
+        if not 0 <= offset <= held:
+            raise ValueError(f"QuantizedKVCache meta_state names {offset} tokens of {held}")
+        self.group_size, self.bits = _check_group(group), _check_bits(bits)
+        self.key_bits, self.val_bits = _check_bits(kb), _check_bits(vb)
+        self.offset = offset
+
+    def is_trimmable(self):
+        return True
+
+    def trim(self, n):
+        """Drop the last n tokens; stale rows are overwritten by the next append."""
+        n = min(self.offset, n)
+        self.offset -= n
+        return n
+
+    def make_mask(self, *args, **kwargs):
+        return create_attention_mask(*args, offset=self.offset, **kwargs)
+
+    def empty(self):
+        return self.keys is None
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for s in self.state for t in s)
 
 
 # ---------------------------------------------------------------- masks ----
@@ -620,6 +783,7 @@ def create_attention_mask(N, offset: int = 0, return_array: bool = False,
 def make_prompt_cache(model=None, max_kv_size: Optional[int] = None,
                       turbo_kv_bits: Optional[float] = None, turbo_fp16_layers: int = 1, *,
                       num_layers: Optional[int] = None, fp16_layer_policy: str = "first_last",
+                      kv_bits: Optional[int] = None, kv_group_size: int = 64,
                       **turbo_kwargs) -> List[Any]:
     """Per-layer cache list (cache.py:15-68).
 
@@ -629,7 +793,19 @@ def make_prompt_cache(model=None, max_kv_size: Optional[int] = None,
     ``TurboQuantKVCache``.  Models with ``make_cache`` get every ``KVCache``
     entry replaced and ``turbo_fp16_layers`` ignored, as in the reference.
     ``num_layers`` stands in for ``len(model.layers)`` when no model is given.
+    With ``kv_bits`` instead, every layer (every ``KVCache`` entry of
+    ``make_cache``) keeps a ``QuantizedKVCache`` of that width in groups of
+    ``kv_group_size``; ``key_bits`` / ``val_bits`` may set a side's own.
     """
+    if kv_bits is not None:
+        if turbo_kv_bits is not None:
+            raise ValueError("kv_bits and turbo_kv_bits name two different caches")
+        if max_kv_size is not None:
+            raise NotImplementedError("RotatingKVCache (max_kv_size) is outside this library's scope")
+        def affine(): return QuantizedKVCache(group_size=kv_group_size, bits=kv_bits, **turbo_kwargs)
+        if model is not None and hasattr(model, "make_cache"):
+            return [affine() if isinstance(c, KVCache) else c for c in model.make_cache()]
+        return [affine() for _ in range(num_layers if num_layers is not None else len(model.layers))]
     if model is not None and hasattr(model, "make_cache"):
         caches = model.make_cache()
         if turbo_kv_bits is not None:
@@ -699,7 +875,8 @@ def _tree_unflatten(items):
     return fix(root)
 
 
-_ALLOWED_CACHE_CLASSES = {"KVCache", "TurboQuantKVCache", "BatchKVCache", "BatchTurboQuantKVCache"}
+_ALLOWED_CACHE_CLASSES = {"KVCache", "TurboQuantKVCache", "QuantizedKVCache", "BatchKVCache",
+                          "BatchTurboQuantKVCache"}
 
 
 def save_prompt_cache(file_name: str, cache: List[Any], metadata: Dict[str, str] = {}):
@@ -758,6 +935,10 @@ def load_prompt_cache(file_name: str, return_metadata: bool = False, device=None
                 st = (kst, TurboQuantMSEState(*st[1]))
             else:
                 st = []
+        elif cls_name == "QuantizedKVCache":
+            cls = QuantizedKVCache
+            ok = isinstance(st, list) and len(st) == 2 and all(isinstance(s, list) and len(s) == 2 for s in st)
+            st = tuple(AffineState(*s) for s in st) if ok else []
         elif cls_name in ("BatchTurboQuantKVCache", "BatchKVCache"):
             # (keys, values, offset, left_padding); absent keys were not saved
             st = list(st) + [[]] * (4 - len(st)) if isinstance(st, list) else [[]] * 4

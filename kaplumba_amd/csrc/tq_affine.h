@@ -1,0 +1,71 @@
+// Group-affine cache: what its kernels share.
+//
+// A row of dim coordinates is stored as dim * bits / 32 words (bits 4 or 8, coordinate i at bits i * bits, least
+// significant first) and one (scale, bias) pair per group of 32, 64 or 128 coordinates, in the type T of the
+// vectors: coordinate i stands for scale * code_i + bias.
+#pragma once
+
+#include "tq_common.h"
+
+namespace tq {
+
+struct AffineAttnParams {
+  const void* q;
+  int64_t q_sb, q_sh, q_sl;
+  const uint32_t* k_codes;
+  const void* k_params;
+  const uint32_t* v_codes;
+  const void* v_params;
+  const int32_t* starts;
+  const int32_t* lens;
+  const void* mask;
+  int64_t mask_s[5];
+  int mask_kind;
+  int causal;
+  int64_t capacity, max_tokens;
+  int B, Hkv, R, L;       // R query heads a kv head
+  int rows;               // R * L; row = l * R + r
+  int k_dim, v_dim;
+  int group;
+  float scale;            // of the scores, times log2(e)
+  int splits;
+  int64_t split_tokens;   // tokens a split takes of every sequence
+  void* out;
+  float* part_o;          // [B * Hkv * rows, splits, v_dim]
+  float* part_ml;         // [B * Hkv * rows, splits, 2]: running maximum (base 2), sum
+};
+
+// Tokens [start, end) of sequence b, as the device arrays say, within the cache.
+__device__ __forceinline__ void affine_range(const AffineAttnParams& p, int b, int64_t& start, int64_t& end) {
+  end = p.lens ? min(static_cast<int64_t>(p.lens[b]), p.max_tokens) : p.max_tokens;
+  start = p.starts ? max(static_cast<int64_t>(p.starts[b]), static_cast<int64_t>(0)) : 0;
+  if (end < start) end = start;
+}
+
+// The score x (base 2 units) of query row (b, g, r, l) for cache row t under the array mask.  An added
+// -FLT_MAX keeps its place above -inf, as in the other attention kernels.
+__device__ __forceinline__ float affine_mask(const AffineAttnParams& p, int64_t off, float x) {
+  if (p.mask_kind == TQ_MASK_BOOL) return static_cast<const uint8_t*>(p.mask)[off] ? x : -FLT_MAX;
+  const float m = p.mask_kind == TQ_MASK_ADD_F32   ? static_cast<const float*>(p.mask)[off]
+                  : p.mask_kind == TQ_MASK_ADD_F16 ? f16_bits_to_f32(static_cast<const uint16_t*>(p.mask)[off])
+                                                   : bf16_bits_to_f32(static_cast<const uint16_t*>(p.mask)[off]);
+  if (m == -INFINITY) return m;  // also where the score is not finite
+  const float t = __builtin_fmaf(m, 1.44269504088896341f, x);
+  return t == -INFINITY ? -FLT_MAX : t;
+}
+
+// (scale, bias) of one group.
+template <int DT>
+__device__ __forceinline__ float2 affine_pair(const void* params, int64_t i) {
+  if constexpr (DT == TQ_DTYPE_F32) {
+    return static_cast<const float2*>(params)[i];
+  } else {
+    const uint32_t u = static_cast<const uint32_t*>(params)[i];
+    if constexpr (DT == TQ_DTYPE_F16)
+      return make_float2(f16_bits_to_f32(u & 0xffffu), f16_bits_to_f32(u >> 16));
+    else
+      return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+}
+
+}  // namespace tq

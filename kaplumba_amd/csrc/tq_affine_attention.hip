@@ -1,0 +1,319 @@
+// Attention over the group-affine cache: entry points, the vector kernel and the merge.
+#include <algorithm>
+
+#include "tq_affine.h"
+
+namespace tq {
+namespace {
+
+constexpr int kVecRows = 4;     // query rows a workgroup of the vector kernel takes
+constexpr int kVecTokens = 64;  // tokens a step
+constexpr int kMaxDim = 512;
+
+template <int DT, int BITS>
+__device__ __forceinline__ float code_of(const uint32_t* row, int d) {
+  constexpr int kPer = 32 / BITS;
+  return static_cast<float>((row[d / kPer] >> (d % kPer * BITS)) & ((1u << BITS) - 1u));
+}
+
+// S = scale * sum_g (s_g (q . c)_g + b_g sum(q)_g), an online softmax per row, O = sum p (s c + b): all in f32.
+// Wave = a quarter of the 32-coordinate blocks and lane = token for the scores, wave = row for the softmax,
+// thread = coordinate for the values.  Bound by its vector instructions, about rows * (Dk + Dv) multiply-adds a
+// token; it serves the dims that the matrix-core kernels do not take.
+template <int DT, int KB, int VB>
+__global__ __launch_bounds__(256) void affine_vector_kernel(const AffineAttnParams p) {
+  __shared__ float qs[kVecRows][kMaxDim];
+  __shared__ float qsum[kVecRows][kMaxDim / 32];
+  __shared__ float part[4][kVecRows][kVecTokens];
+  __shared__ float pr[kVecRows][kVecTokens];
+  __shared__ float alpha[kVecRows];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int split = blockIdx.x % p.splits;
+  const int blk = blockIdx.x / p.splits;
+  const int row_blocks = (p.rows + kVecRows - 1) / kVecRows;
+  const int bh = blk / row_blocks, row0 = (blk % row_blocks) * kVecRows;
+  const int b = bh / p.Hkv, h = bh % p.Hkv;
+
+  for (int i = tid; i < kVecRows * p.k_dim; i += 256) {
+    const int s = i / p.k_dim, d = i % p.k_dim;
+    const int row = min(row0 + s, p.rows - 1);
+    qs[s][d] = load_elem<DT>(p.q, b * p.q_sb + (static_cast<int64_t>(h) * p.R + row % p.R) * p.q_sh +
+                                      static_cast<int64_t>(row / p.R) * p.q_sl + d);
+  }
+  __syncthreads();
+  const int blocks32 = p.k_dim / 32;
+  for (int i = tid; i < kVecRows * blocks32; i += 256) {
+    const int s = i / blocks32, c = i % blocks32;
+    float t = 0.f;
+    for (int d = 0; d < 32; ++d) t += qs[s][c * 32 + d];
+    qsum[s][c] = t;
+  }
+  __syncthreads();
+
+  int64_t start, end;
+  affine_range(p, b, start, end);
+  const int64_t t0 = start + split * p.split_tokens;
+  const int64_t t1 = min(end, t0 + p.split_tokens);
+  const int kw = p.k_dim * KB / 32, vw = p.v_dim * VB / 32;
+  const int kg = p.k_dim / p.group, vg = p.v_dim / p.group;
+  const int64_t base = static_cast<int64_t>(bh) * p.capacity;
+  const int my_row = min(row0 + wave, p.rows - 1);
+  const int my_l = my_row / p.R, my_r = my_row % p.R;
+  const int64_t lim = p.causal ? end - p.L + my_l : INT64_MAX;
+  float m = -INFINITY, l = 0.f;
+  float acc[kVecRows][2] = {};
+
+  for (int64_t t = t0; t < t1; t += kVecTokens) {
+    const int64_t tok = min(t + lane, t1 - 1);
+    float dot[kVecRows] = {};
+    for (int c = wave; c < blocks32; c += 4) {
+      const uint32_t* row = p.k_codes + (base + tok) * kw + c * KB;
+      const float2 sb = affine_pair<DT>(p.k_params, (base + tok) * kg + c * 32 / p.group);
+      float part32[kVecRows] = {};
+      for (int w = 0; w < KB; ++w) {
+        const uint32_t word = row[w];
+#pragma unroll
+        for (int j = 0; j < 32 / KB; ++j) {
+          const float code = static_cast<float>((word >> (j * KB)) & ((1u << KB) - 1u));
+#pragma unroll
+          for (int s = 0; s < kVecRows; ++s)
+            part32[s] = __builtin_fmaf(qs[s][c * 32 + w * (32 / KB) + j], code, part32[s]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kVecRows; ++s)
+        dot[s] = __builtin_fmaf(sb.x, part32[s], __builtin_fmaf(sb.y, qsum[s][c], dot[s]));
+    }
+#pragma unroll
+    for (int s = 0; s < kVecRows; ++s) part[wave][s][lane] = dot[s];
+    __syncthreads();
+    {
+      float x = (part[0][wave][lane] + part[1][wave][lane]) + (part[2][wave][lane] + part[3][wave][lane]);
+      x *= p.scale;
+      if (p.mask_kind != TQ_MASK_NONE)
+        x = affine_mask(p, b * p.mask_s[0] + h * p.mask_s[1] + my_r * p.mask_s[2] + my_l * p.mask_s[3] + tok * p.mask_s[4], x);
+      if (tok > lim && x != -INFINITY) x = -FLT_MAX;
+      if (t + lane >= t1) x = -INFINITY;
+      float mx = x;
+      for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      const float m_new = fmaxf(m, mx);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      const float w = exp2f(x - ref);
+      const float a = exp2f(m - ref);
+      float sum = w;
+      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      l = l * a + sum;
+      m = m_new;
+      pr[wave][lane] = w;
+      if (lane == 0) alpha[wave] = a;
+    }
+    __syncthreads();
+    const int n = static_cast<int>(min(static_cast<int64_t>(kVecTokens), t1 - t));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int d = tid + e * 256;
+      if (d >= p.v_dim) break;
+#pragma unroll
+      for (int s = 0; s < kVecRows; ++s) acc[s][e] *= alpha[s];
+      for (int i = 0; i < n; ++i) {
+        const float2 sb = affine_pair<DT>(p.v_params, (base + t + i) * vg + d / p.group);
+        const float v = __builtin_fmaf(sb.x, code_of<DT, VB>(p.v_codes + (base + t + i) * vw, d), sb.y);
+#pragma unroll
+        for (int s = 0; s < kVecRows; ++s) {
+          const float w = pr[s][i];
+          acc[s][e] = w == 0.f ? acc[s][e] : __builtin_fmaf(w, v, acc[s][e]);  // what a row masks may be NaN
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int s = 0; s < kVecRows; ++s) {
+    const int row = row0 + s;
+    if (row >= p.rows) break;
+    const int64_t at = (static_cast<int64_t>(bh) * p.rows + row) * p.splits + split;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * 256 < p.v_dim) p.part_o[at * p.v_dim + tid + e * 256] = acc[s][e];
+  }
+  if (lane == 0 && row0 + wave < p.rows) {
+    const int64_t at = (static_cast<int64_t>(bh) * p.rows + row0 + wave) * p.splits + split;
+    p.part_ml[2 * at] = m;
+    p.part_ml[2 * at + 1] = l;
+  }
+}
+
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's splits; a row without a token, or whose every
+// score is -inf, gives zeros.  One workgroup a row: every thread finds M and the sum itself (the splits' pairs are
+// a few cache lines), then takes coordinates.
+template <int DT>
+__global__ __launch_bounds__(128) void affine_merge_kernel(const AffineAttnParams p) {
+  const int64_t at = blockIdx.x;  // (b, h, row)
+  const int row = static_cast<int>(at % p.rows);
+  const int64_t bh = at / p.rows;
+  const float* ml = p.part_ml + at * p.splits * 2;
+  float M = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, ml[2 * s]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float sum = 0.f;
+  for (int s = 0; s < p.splits; ++s) sum += exp2f(ml[2 * s] - ref) * ml[2 * s + 1];
+  const int64_t head = bh * p.R + row % p.R;  // b * Hq + query head
+  const int64_t to = (head * p.L + row / p.R) * p.v_dim;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int d = threadIdx.x; d < p.v_dim; d += 128) {
+    float o = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float w = exp2f(ml[2 * s] - ref);
+      const float x = p.part_o[(at * p.splits + s) * p.v_dim + d];
+      o = w == 0.f ? o : __builtin_fmaf(w, x, o);
+    }
+    store_elem<DT>(p.out, to + d, o * inv);
+  }
+}
+
+int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
+
+struct Plan {
+  int splits;
+  int64_t split_tokens;
+};
+
+constexpr int64_t kVecTarget = 512;  // workgroups of the vector kernel to aim at: two a CU
+
+// Splits of the vector kernel: about kVecTarget workgroups, at least 64 tokens each.
+Plan vector_plan(int64_t blocks, int64_t max_tokens) {
+  const int64_t most = (max_tokens + kVecTokens - 1) / kVecTokens;
+  const int64_t s = std::max<int64_t>(1, std::min((kVecTarget + blocks - 1) / blocks, most));
+  const int64_t per = std::max<int64_t>(1, ((max_tokens + s - 1) / s + kVecTokens - 1) / kVecTokens) * kVecTokens;
+  return {static_cast<int>(std::max<int64_t>(1, (max_tokens + per - 1) / per)), per};
+}
+
+int64_t rows_of(int B, int Hq, int L) { return static_cast<int64_t>(B) * Hq * L; }
+
+Plan plan_for(int B, int Hq, int Hkv, int L, int64_t max_tokens) {
+  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * L;
+  return vector_plan(static_cast<int64_t>(B) * Hkv * ((rows + kVecRows - 1) / kVecRows), max_tokens);
+}
+
+// Rows times splits of any plan with at most these sequences, queries and tokens: with n workgroups of kVecRows rows
+// there are at most kVecTarget / n + 1 splits.
+int64_t most_partials(int B, int Hq, int L, int64_t max_tokens) {
+  const int64_t rows = rows_of(B, Hq, L), most = std::max<int64_t>(1, (max_tokens + kVecTokens - 1) / kVecTokens);
+  return std::min(rows * most, kVecTarget * kVecRows + rows);
+}
+
+int64_t workspace_bytes(int B, int Hq, int L, int v_dim, int64_t max_tokens) {
+  const int64_t n = most_partials(B, Hq, L, max_tokens);
+  return align256(n * 8) + align256(n * v_dim * 4);
+}
+
+template <int DT>
+void launch_vector(const AffineAttnParams& p, int k_bits, int v_bits, unsigned blocks, hipStream_t stream) {
+  if (k_bits == 4 && v_bits == 4)
+    affine_vector_kernel<DT, 4, 4><<<blocks, 256, 0, stream>>>(p);
+  else if (k_bits == 8 && v_bits == 4)
+    affine_vector_kernel<DT, 8, 4><<<blocks, 256, 0, stream>>>(p);
+  else if (k_bits == 8)
+    affine_vector_kernel<DT, 8, 8><<<blocks, 256, 0, stream>>>(p);
+  else
+    affine_vector_kernel<DT, 4, 8><<<blocks, 256, 0, stream>>>(p);
+}
+
+template <int DT>
+void launch_merge(const AffineAttnParams& p, unsigned rows, hipStream_t stream) {
+  affine_merge_kernel<DT><<<rows, 128, 0, stream>>>(p);
+}
+
+bool dims_ok(int k_dim, int v_dim, int group) {
+  return (group == 32 || group == 64 || group == 128) && k_dim >= group && v_dim >= group && k_dim <= kMaxDim &&
+         v_dim <= kMaxDim && k_dim % group == 0 && v_dim % group == 0;
+}
+
+}  // namespace
+}  // namespace tq
+
+using namespace tq;
+
+extern "C" {
+
+int64_t tq_attention_affine_workspace_size(int B, int Hq, int Hkv, int L, int k_dim, int v_dim, int64_t max_tokens) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || Hq % Hkv || max_tokens < 0 || k_dim <= 0 || v_dim <= 0 ||
+      k_dim > kMaxDim || v_dim > kMaxDim)
+    return 0;
+  return workspace_bytes(B, Hq, L, v_dim, max_tokens);
+}
+
+int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int L, int k_dim, int v_dim,
+                        int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_l, float scale,
+                        const uint32_t* k_codes, const void* k_params, int k_bits, const uint32_t* v_codes,
+                        const void* v_params, int v_bits, int group, int64_t capacity, int64_t max_tokens,
+                        const int32_t* seq_starts, const int32_t* seq_lens, int causal, const void* mask,
+                        int mask_kind, const int64_t* mask_strides, void* out, void* workspace,
+                        int64_t workspace_bytes_given, void* stream) {
+  if (q_dtype < TQ_DTYPE_F32 || q_dtype > TQ_DTYPE_BF16)
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: q_dtype %d", q_dtype);
+  if (B < 0 || Hq < 0 || L < 0 || Hkv < 1 || Hq % Hkv)
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: bad sizes B=%d, heads %d over %d kv heads, L=%d", B, Hq, Hkv, L);
+  if ((k_bits != 4 && k_bits != 8) || (v_bits != 4 && v_bits != 8))
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: bits %d / %d are not 4 or 8", k_bits, v_bits);
+  if (!dims_ok(k_dim, v_dim, group))
+    return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: head dims %d / %d in groups of %d (multiples of a group of 32, 64 or 128, to %d)",
+                k_dim, v_dim, group, kMaxDim);
+  if (capacity < 0 || capacity > INT32_MAX || max_tokens < 0 || max_tokens > capacity)
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: %lld tokens of a capacity of %lld", static_cast<long long>(max_tokens),
+                static_cast<long long>(capacity));
+  if (mask_kind < TQ_MASK_NONE || mask_kind > TQ_MASK_ADD_BF16)
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: mask_kind %d", mask_kind);
+  if (mask_kind != TQ_MASK_NONE && max_tokens > 0 && (!mask || !mask_strides))
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: a mask without its pointer or strides");
+  const int64_t rows64 = static_cast<int64_t>(Hq / Hkv) * L;
+  if (rows64 > INT32_MAX / 4 || rows_of(B, Hq, L) > INT32_MAX / 4)
+    return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld query rows", static_cast<long long>(rows_of(B, Hq, L)));
+  if (B == 0 || Hq == 0 || L == 0) return TQ_OK;
+  if (!q || !out || (max_tokens > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: null pointer");
+  const int64_t need = workspace_bytes(B, Hq, L, v_dim, max_tokens);
+  if (!workspace || workspace_bytes_given < need)
+    return fail(TQ_ERR_WORKSPACE, "tq_attention_affine: workspace of %lld bytes, %lld needed",
+                static_cast<long long>(workspace_bytes_given), static_cast<long long>(need));
+
+  const Plan pl = plan_for(B, Hq, Hkv, L, max_tokens);
+  AffineAttnParams p{};
+  p.q = q;
+  p.q_sb = q_stride_b, p.q_sh = q_stride_h, p.q_sl = q_stride_l;
+  p.k_codes = k_codes, p.k_params = k_params, p.v_codes = v_codes, p.v_params = v_params;
+  p.starts = seq_starts, p.lens = seq_lens;
+  p.mask = mask, p.mask_kind = mask_kind;
+  if (mask_kind != TQ_MASK_NONE && mask_strides)
+    for (int i = 0; i < 5; ++i) p.mask_s[i] = mask_strides[i];
+  p.causal = causal;
+  p.capacity = capacity, p.max_tokens = max_tokens;
+  p.B = B, p.Hkv = Hkv, p.R = Hq / Hkv, p.L = L;
+  p.rows = static_cast<int>(rows64);
+  p.k_dim = k_dim, p.v_dim = v_dim, p.group = group;
+  p.scale = scale * 1.44269504088896341f;
+  p.splits = pl.splits, p.split_tokens = pl.split_tokens;
+  p.out = out;
+  const int64_t n = rows_of(B, Hq, L) * pl.splits;
+  p.part_ml = static_cast<float*>(workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(n * 8));
+
+  const int64_t blocks = static_cast<int64_t>(B) * Hkv * ((p.rows + kVecRows - 1) / kVecRows) * pl.splits;
+  if (blocks > INT32_MAX) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const unsigned out_rows = static_cast<unsigned>(rows_of(B, Hq, L));
+  if (q_dtype == TQ_DTYPE_F32) {
+    launch_vector<TQ_DTYPE_F32>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
+    launch_merge<TQ_DTYPE_F32>(p, out_rows, st);
+  } else if (q_dtype == TQ_DTYPE_F16) {
+    launch_vector<TQ_DTYPE_F16>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
+    launch_merge<TQ_DTYPE_F16>(p, out_rows, st);
+  } else {
+    launch_vector<TQ_DTYPE_BF16>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
+    launch_merge<TQ_DTYPE_BF16>(p, out_rows, st);
+  }
+  return check_launch("tq_attention_affine");
+}
+
+}  // extern "C"

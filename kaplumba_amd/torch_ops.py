@@ -26,17 +26,24 @@ Operators:
   prod_dequantize(norms, mse_indices, residual_norms, qjl_signs, dim, bits, seed) -> f32
   attention_prod(q, <Prod key state>, v_norms, v_idx, k_dim, k_bits, k_seed, <value codec>,
                  scale, causal, seq_lens?, seq_starts?, mask?) -> (B, Hq, L, Dv)
+  norm_rope(q, k, positions?, start, inv_freq?, axis?, q_weight?, k_weight?, eps, pairs, factor) -> (q, k)
+  append_affine_kv(k, v, k_codes!, k_params!, v_codes!, v_params!, offset, group_size)
+  dequantize_affine(codes, params, group_size, dtype) -> (B, H, T, dim)
+  attention_affine(q, k_codes, k_params, v_codes, v_params, group_size, scale, causal,
+                   seq_lens?, seq_starts?, mask?) -> (B, Hq, L, Dv)
 (``!``: written in place.)
 """
 from __future__ import annotations
 
 import functools
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
+from . import affine
 from . import ops
 from . import prod
+from . import rope
 
 
 @functools.lru_cache(maxsize=None)
@@ -182,3 +189,56 @@ def _(queries, norms, mse_indices, residual_norms, qjl_signs, v_norms, v_idx, k_
       v_dim, v_bits, v_seed, v_rotation, v_codebook, scale, causal, seq_lens, seq_starts, mask):
     B, Hq, L, _ = queries.shape
     return queries.new_empty((B, Hq, L, v_dim))
+
+
+@torch.library.custom_op("kaplumba::norm_rope", mutates_args=())
+def norm_rope(queries: torch.Tensor, keys: torch.Tensor, positions: Optional[torch.Tensor], start: int,
+              inv_freq: Optional[torch.Tensor], axis: Optional[torch.Tensor], q_weight: Optional[torch.Tensor],
+              k_weight: Optional[torch.Tensor], eps: float, pairs: str,
+              factor: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    return rope.norm_rope(queries, keys, start if positions is None else positions, inv_freq, axis=axis,
+                          q_weight=q_weight, k_weight=k_weight, eps=eps, pairs=pairs, factor=factor, _direct=True)
+
+
+@norm_rope.register_fake
+def _(queries, keys, positions, start, inv_freq, axis, q_weight, k_weight, eps, pairs, factor):
+    return queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+
+
+@torch.library.custom_op("kaplumba::append_affine_kv", mutates_args=("k_codes", "k_params", "v_codes", "v_params"))
+def append_affine_kv(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tensor,
+                     v_codes: torch.Tensor, v_params: torch.Tensor, offset: int, group_size: int) -> None:
+    affine.append_affine_kv(k, v, affine.AffineState(k_codes, k_params), affine.AffineState(v_codes, v_params), offset,
+                            group_size, _direct=True)
+
+
+@append_affine_kv.register_fake
+def _(k, v, k_codes, k_params, v_codes, v_params, offset, group_size):
+    return None
+
+
+@torch.library.custom_op("kaplumba::dequantize_affine", mutates_args=())
+def dequantize_affine(codes: torch.Tensor, params: torch.Tensor, group_size: int, dtype: torch.dtype) -> torch.Tensor:
+    return affine.dequantize_affine(affine.AffineState(codes, params), group_size, dtype, _direct=True)
+
+
+@dequantize_affine.register_fake
+def _(codes, params, group_size, dtype):
+    B, H, T, groups, _ = params.shape
+    return params.new_empty((B, H, T, groups * group_size), dtype=dtype)
+
+
+@torch.library.custom_op("kaplumba::attention_affine", mutates_args=())
+def attention_affine(queries: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor,
+                     v_params: torch.Tensor, group_size: int, scale: float, causal: bool,
+                     seq_lens: Optional[torch.Tensor], seq_starts: Optional[torch.Tensor],
+                     mask: Optional[torch.Tensor]) -> torch.Tensor:
+    return affine.attention_affine(queries, affine.AffineState(k_codes, k_params), affine.AffineState(v_codes, v_params),
+                                   group_size, scale, causal, seq_lens=seq_lens, seq_starts=seq_starts, mask=mask,
+                                   _direct=True)
+
+
+@attention_affine.register_fake
+def _(queries, k_codes, k_params, v_codes, v_params, group_size, scale, causal, seq_lens, seq_starts, mask):
+    B, Hq, L, _ = queries.shape
+    return queries.new_empty((B, Hq, L, v_params.shape[3] * group_size))
