@@ -35,6 +35,17 @@ struct AffineAttnParams {
   float* part_ml;         // [B * Hkv * rows, splits, 2]: running maximum (base 2), sum
 };
 
+// Which instantiation of the few-rows kernel (tq_affine_rows.h) takes a call: head dims up to `dim`, exactly it
+// where `full`, and `rows` query rows a workgroup.
+struct RowsChoice {
+  int dim, rows;
+  bool full;
+};
+
+int launch_rows_k4v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
+int launch_rows_k8v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
+int launch_rows_k8v8(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
+
 // Tokens [start, end) of sequence b, as the device arrays say, within the cache.
 __device__ __forceinline__ void affine_range(const AffineAttnParams& p, int b, int64_t& start, int64_t& end) {
   end = p.lens ? min(static_cast<int64_t>(p.lens[b]), p.max_tokens) : p.max_tokens;

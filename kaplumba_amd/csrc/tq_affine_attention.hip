@@ -1,7 +1,7 @@
 // Attention over the group-affine cache: entry points, the vector kernel and the merge.
 #include <algorithm>
 
-#include "tq_affine.h"
+#include "tq_affine_rows.h"
 
 namespace tq {
 namespace {
@@ -145,30 +145,51 @@ __global__ __launch_bounds__(256) void affine_vector_kernel(const AffineAttnPara
 }
 
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over a row's splits; a row without a token, or whose every
-// score is -inf, gives zeros.  One workgroup a row: every thread finds M and the sum itself (the splits' pairs are
-// a few cache lines), then takes coordinates.
+// score is -inf, gives zeros.  One workgroup a row: its waves take splits and its lanes four coordinates each, then
+// the waves' sums meet in LDS.
 template <int DT>
-__global__ __launch_bounds__(128) void affine_merge_kernel(const AffineAttnParams p) {
+__global__ __launch_bounds__(256) void affine_merge_kernel(const AffineAttnParams p) {
+  __shared__ float part[4][kMaxDim + 1];
   const int64_t at = blockIdx.x;  // (b, h, row)
   const int row = static_cast<int>(at % p.rows);
   const int64_t bh = at / p.rows;
-  const float* ml = p.part_ml + at * p.splits * 2;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at * p.splits;
   float M = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, ml[2 * s]);
+  for (int s = lane; s < p.splits; s += 64) M = fmaxf(M, ml[s].x);
+  for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
   const float ref = M == -INFINITY ? 0.f : M;
+  float4 o[2] = {};
   float sum = 0.f;
-  for (int s = 0; s < p.splits; ++s) sum += exp2f(ml[2 * s] - ref) * ml[2 * s + 1];
+  for (int s = wave; s < p.splits; s += 4) {
+    const float2 t = ml[s];
+    const float w = __builtin_amdgcn_exp2f(t.x - ref);
+    sum = __builtin_fmaf(w, t.y, sum);
+    const float4* from = reinterpret_cast<const float4*>(p.part_o + (at * p.splits + s) * p.v_dim);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if ((lane + 64 * e) * 4 >= p.v_dim) break;
+      const float4 x = from[lane + 64 * e];
+      if (w != 0.f) {
+        o[e].x = __builtin_fmaf(w, x.x, o[e].x), o[e].y = __builtin_fmaf(w, x.y, o[e].y);
+        o[e].z = __builtin_fmaf(w, x.z, o[e].z), o[e].w = __builtin_fmaf(w, x.w, o[e].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = (lane + 64 * e) * 4;
+    if (d >= p.v_dim) break;
+    part[wave][d] = o[e].x, part[wave][d + 1] = o[e].y, part[wave][d + 2] = o[e].z, part[wave][d + 3] = o[e].w;
+  }
+  if (lane == 0) part[wave][kMaxDim] = sum;
+  __syncthreads();
+  const float all = (part[0][kMaxDim] + part[1][kMaxDim]) + (part[2][kMaxDim] + part[3][kMaxDim]);
   const int64_t head = bh * p.R + row % p.R;  // b * Hq + query head
   const int64_t to = (head * p.L + row / p.R) * p.v_dim;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = threadIdx.x; d < p.v_dim; d += 128) {
-    float o = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float w = exp2f(ml[2 * s] - ref);
-      const float x = p.part_o[(at * p.splits + s) * p.v_dim + d];
-      o = w == 0.f ? o : __builtin_fmaf(w, x, o);
-    }
-    store_elem<DT>(p.out, to + d, o * inv);
+  for (int d = threadIdx.x; d < p.v_dim; d += 256) {
+    const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+    store_elem<DT>(p.out, to + d, all == 0.f ? 0.f : x / all);
   }
 }
 
@@ -179,28 +200,39 @@ struct Plan {
   int64_t split_tokens;
 };
 
-constexpr int64_t kVecTarget = 512;  // workgroups of the vector kernel to aim at: two a CU
+constexpr int64_t kVecTarget = 512;     // workgroups of the vector kernel to aim at: two a CU
+constexpr int64_t kRowsTarget = 256;    // of the few-rows kernel: eight waves, two a SIMD, on every CU
+constexpr int64_t kRaggedTarget = 1024; // where sequences end at different tokens: finer, so that CUs share the long ones
+constexpr int kRowsTokens = 512;        // tokens of one step of a workgroup's eight waves
 
-// Splits of the vector kernel: about kVecTarget workgroups, at least 64 tokens each.
-Plan vector_plan(int64_t blocks, int64_t max_tokens) {
-  const int64_t most = (max_tokens + kVecTokens - 1) / kVecTokens;
-  const int64_t s = std::max<int64_t>(1, std::min((kVecTarget + blocks - 1) / blocks, most));
-  const int64_t per = std::max<int64_t>(1, ((max_tokens + s - 1) / s + kVecTokens - 1) / kVecTokens) * kVecTokens;
+// A split for every `unit` tokens at most, and about `target` workgroups in all.
+Plan plan_splits(int64_t blocks, int64_t max_tokens, int64_t target, int unit) {
+  const int64_t most = (max_tokens + unit - 1) / unit;
+  const int64_t s = std::max<int64_t>(1, std::min(target / blocks, most));
+  const int64_t per = std::max<int64_t>(1, ((max_tokens + s - 1) / s + unit - 1) / unit) * unit;
   return {static_cast<int>(std::max<int64_t>(1, (max_tokens + per - 1) / per)), per};
 }
 
 int64_t rows_of(int B, int Hq, int L) { return static_cast<int64_t>(B) * Hq * L; }
 
-Plan plan_for(int B, int Hq, int Hkv, int L, int64_t max_tokens) {
-  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * L;
-  return vector_plan(static_cast<int64_t>(B) * Hkv * ((rows + kVecRows - 1) / kVecRows), max_tokens);
+// The few-rows kernel takes 16-bit types and head dims to 256 (f32 and larger dims: the vector kernel).
+bool rows_kernel(int dtype, int k_dim, int v_dim, int k_bits, int v_bits) {
+  return dtype != TQ_DTYPE_F32 && k_dim <= 256 && v_dim <= 256 && !(k_bits == 4 && v_bits == 8);
 }
 
-// Rows times splits of any plan with at most these sequences, queries and tokens: with n workgroups of kVecRows rows
-// there are at most kVecTarget / n + 1 splits.
+RowsChoice rows_choice(int64_t rows, int k_dim, int v_dim, int v_bits, int group) {
+  RowsChoice r;
+  r.full = k_dim == v_dim && (k_dim == 64 || k_dim == 128 || k_dim == 256) && group <= 64;
+  r.dim = r.full ? k_dim : std::max(k_dim, v_dim) <= 128 ? 128 : 256;
+  r.rows = r.full && rows <= 4 ? 4 : rows_large(v_bits, r.dim, group);
+  return r;
+}
+
+// Rows times splits of any plan with at most these sequences, queries and tokens: n workgroups of k rows have at most
+// target / n splits, and at least one.
 int64_t most_partials(int B, int Hq, int L, int64_t max_tokens) {
   const int64_t rows = rows_of(B, Hq, L), most = std::max<int64_t>(1, (max_tokens + kVecTokens - 1) / kVecTokens);
-  return std::min(rows * most, kVecTarget * kVecRows + rows);
+  return std::min(rows * most, std::max(kVecTarget * kVecRows, kRaggedTarget * 16) + rows);
 }
 
 int64_t workspace_bytes(int B, int Hq, int L, int v_dim, int64_t max_tokens) {
@@ -218,11 +250,6 @@ void launch_vector(const AffineAttnParams& p, int k_bits, int v_bits, unsigned b
     affine_vector_kernel<DT, 8, 8><<<blocks, 256, 0, stream>>>(p);
   else
     affine_vector_kernel<DT, 4, 8><<<blocks, 256, 0, stream>>>(p);
-}
-
-template <int DT>
-void launch_merge(const AffineAttnParams& p, unsigned rows, hipStream_t stream) {
-  affine_merge_kernel<DT><<<rows, 128, 0, stream>>>(p);
 }
 
 bool dims_ok(int k_dim, int v_dim, int group) {
@@ -278,7 +305,17 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
     return fail(TQ_ERR_WORKSPACE, "tq_attention_affine: workspace of %lld bytes, %lld needed",
                 static_cast<long long>(workspace_bytes_given), static_cast<long long>(need));
 
-  const Plan pl = plan_for(B, Hq, Hkv, L, max_tokens);
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) |
+       static_cast<uintptr_t>((q_stride_b | q_stride_h | q_stride_l) * (q_dtype == TQ_DTYPE_F32 ? 4 : 2))) & 15)
+    return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: queries, their strides and the codes must be 16-byte aligned");
+
+  const bool by_rows = rows_kernel(q_dtype, k_dim, v_dim, k_bits, v_bits);
+  const RowsChoice rc = rows_choice(rows64, k_dim, v_dim, v_bits, group);
+  const int block_rows = by_rows ? rc.rows : kVecRows;
+  const int64_t blocks1 = static_cast<int64_t>(B) * Hkv * ((rows64 + block_rows - 1) / block_rows);
+  const bool ragged = seq_lens || seq_starts;
+  const Plan pl = by_rows ? plan_splits(blocks1, max_tokens, ragged ? kRaggedTarget : kRowsTarget, kRowsTokens)
+                          : plan_splits(blocks1, max_tokens, kVecTarget, kVecTokens);
   AffineAttnParams p{};
   p.q = q;
   p.q_sb = q_stride_b, p.q_sh = q_stride_h, p.q_sl = q_stride_l;
@@ -299,20 +336,29 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   p.part_ml = static_cast<float*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + align256(n * 8));
 
-  const int64_t blocks = static_cast<int64_t>(B) * Hkv * ((p.rows + kVecRows - 1) / kVecRows) * pl.splits;
-  if (blocks > INT32_MAX) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
+  const int64_t blocks = blocks1 * pl.splits;
+  if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned out_rows = static_cast<unsigned>(rows_of(B, Hq, L));
-  if (q_dtype == TQ_DTYPE_F32) {
-    launch_vector<TQ_DTYPE_F32>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
-    launch_merge<TQ_DTYPE_F32>(p, out_rows, st);
+  const unsigned n_blocks = static_cast<unsigned>(blocks);
+  if (by_rows) {
+    const int rc_launch = k_bits == 4   ? launch_rows_k4v4(p, rc, q_dtype, st)
+                          : v_bits == 4 ? launch_rows_k8v4(p, rc, q_dtype, st)
+                                        : launch_rows_k8v8(p, rc, q_dtype, st);
+    if (rc_launch != TQ_OK || pl.splits == 1) return rc_launch;
+  } else if (q_dtype == TQ_DTYPE_F32) {
+    launch_vector<TQ_DTYPE_F32>(p, k_bits, v_bits, n_blocks, st);
   } else if (q_dtype == TQ_DTYPE_F16) {
-    launch_vector<TQ_DTYPE_F16>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
-    launch_merge<TQ_DTYPE_F16>(p, out_rows, st);
+    launch_vector<TQ_DTYPE_F16>(p, k_bits, v_bits, n_blocks, st);
   } else {
-    launch_vector<TQ_DTYPE_BF16>(p, k_bits, v_bits, static_cast<unsigned>(blocks), st);
-    launch_merge<TQ_DTYPE_BF16>(p, out_rows, st);
+    launch_vector<TQ_DTYPE_BF16>(p, k_bits, v_bits, n_blocks, st);
   }
+  const unsigned out_rows = static_cast<unsigned>(rows_of(B, Hq, L));
+  if (q_dtype == TQ_DTYPE_F32)
+    affine_merge_kernel<TQ_DTYPE_F32><<<out_rows, 256, 0, st>>>(p);
+  else if (q_dtype == TQ_DTYPE_F16)
+    affine_merge_kernel<TQ_DTYPE_F16><<<out_rows, 256, 0, st>>>(p);
+  else
+    affine_merge_kernel<TQ_DTYPE_BF16><<<out_rows, 256, 0, st>>>(p);
   return check_launch("tq_attention_affine");
 }
 

@@ -81,9 +81,10 @@ def attention(q, k, v, scale, causal=False, seq_lens=None, seq_starts=None, mask
 def attention_tolerance(q, k_params, k_bits, v, want, p, scale, dtype, group, rounded):
     """How far a kernel's output may be from ``want`` (B, Hq, L, Dv), element by element.
 
-    Scores: q and codes meet exactly; a sum of D products in f32 is off by at
-    most (D / 4 + 8) * 2^-24 of the sum of their magnitudes, where a 4-bit code
-    may be carried as 128 + c and the group's sum taken off again.  A score's
+    Scores: q and codes meet exactly (or q off by 2^-27 of its row's largest); a
+    sum of D products in f32 is off by at most (D / 4 + 8) * 2^-24 of the sum of
+    their magnitudes, where a code may be carried as 128 + c (4 bits) or
+    1024 + c (8 bits) and the group's sum taken off again.  A score's
     error dS moves a weight by 2 dS of itself at most (numerator and sum) while
     dS is small.  ``rounded``: keys, weights and values go through the dtype
     (many query rows); independent roundings of half a step u add up to at most
@@ -95,7 +96,7 @@ def attention_tolerance(q, k_params, k_bits, v, want, p, scale, dtype, group, ro
     R = Hq // k_params.shape[1]
     u = half_step(dtype) if rounded and dtype != torch.float32 else 0.0
     kp = torch.nan_to_num(k_params.double(), nan=0.0, posinf=0.0, neginf=0.0).repeat_interleave(R, 1)
-    top = 128 + 15 if k_bits == 4 else 255
+    top = 128 + 15 if k_bits == 4 else 1024 + 255
     size = kp[..., 0].abs() * top + kp[..., 1].abs()                              # (B, Hq, T, groups)
     qa = q.double().abs().unflatten(-1, (-1, group))
     mag = torch.matmul(qa.sum(-1), size.transpose(-1, -2)).amax(-1) * abs(scale)  # (B, Hq, L)
