@@ -46,6 +46,25 @@ int launch_rows_k4v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, 
 int launch_rows_k8v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
 int launch_rows_k8v8(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
 
+// The tokens that rows of the array mask see: the first and one past the last kept one of a row's tokens (those of its
+// sequence, and within its limit under the causal rule), or all of them where it keeps none (such a row weighs them
+// alike).  Rows are told apart by the axes the mask has, and by b and l where windows or the causal rule differ.
+struct MaskRows {
+  int2* range;         // [nb, ng, nr, nl]
+  int nb, ng, nr, nl;
+};
+
+// The many-rows kernel (tq_affine_tile.h): 32 ks key and 16 ct value coordinates; rows a workgroup takes, 0 where no
+// instantiation has these dims.
+constexpr int tile_rows(int k_dim, int v_dim) {
+  return k_dim == v_dim && (k_dim == 64 || k_dim == 96 || k_dim == 128) ? 256
+         : (k_dim == 192 && v_dim == 128) || (k_dim == 256 && v_dim == 256) ? 128 : 0;
+}
+
+int launch_tile_k4v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
+int launch_tile_k8v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
+int launch_tile_k8v8(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
+
 // Tokens [start, end) of sequence b, as the device arrays say, within the cache.
 __device__ __forceinline__ void affine_range(const AffineAttnParams& p, int b, int64_t& start, int64_t& end) {
   end = p.lens ? min(static_cast<int64_t>(p.lens[b]), p.max_tokens) : p.max_tokens;
@@ -65,17 +84,20 @@ __device__ __forceinline__ float affine_mask(const AffineAttnParams& p, int64_t 
   return t == -INFINITY ? -FLT_MAX : t;
 }
 
+// (scale, bias) of a packed pair of 16-bit values.
+template <int DT>
+__device__ __forceinline__ float2 pair16(uint32_t u) {
+  if constexpr (DT == TQ_DTYPE_F16) return make_float2(f16_bits_to_f32(u & 0xffffu), f16_bits_to_f32(u >> 16));
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
 // (scale, bias) of one group.
 template <int DT>
 __device__ __forceinline__ float2 affine_pair(const void* params, int64_t i) {
   if constexpr (DT == TQ_DTYPE_F32) {
     return static_cast<const float2*>(params)[i];
   } else {
-    const uint32_t u = static_cast<const uint32_t*>(params)[i];
-    if constexpr (DT == TQ_DTYPE_F16)
-      return make_float2(f16_bits_to_f32(u & 0xffffu), f16_bits_to_f32(u >> 16));
-    else
-      return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    return pair16<DT>(static_cast<const uint32_t*>(params)[i]);
   }
 }
 

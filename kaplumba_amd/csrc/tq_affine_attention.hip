@@ -193,6 +193,36 @@ __global__ __launch_bounds__(256) void affine_merge_kernel(const AffineAttnParam
   }
 }
 
+// One workgroup a row of MaskRows.
+__global__ __launch_bounds__(256) void affine_mask_range_kernel(const AffineAttnParams p, const MaskRows rows) {
+  __shared__ int lo_s, hi_s;
+  int at = blockIdx.x;
+  const int l = at % rows.nl;
+  at /= rows.nl;
+  const int r = at % rows.nr;
+  at /= rows.nr;
+  const int g = at % rows.ng, b = at / rows.ng;
+  int64_t start, end;
+  affine_range(p, b, start, end);
+  const int64_t seen = p.causal ? max(start, min(end, end - p.L + l + 1)) : end;
+  if (threadIdx.x == 0) lo_s = INT32_MAX, hi_s = 0;
+  __syncthreads();
+  const int64_t from = b * p.mask_s[0] + g * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3];
+  int lo = INT32_MAX, hi = 0;
+  for (int64_t t = start + threadIdx.x; t < seen; t += 256) {
+    // a NaN counts as kept
+    if (!(affine_mask(p, from + t * p.mask_s[4], 0.f) <= (p.mask_kind == TQ_MASK_BOOL ? -FLT_MAX : -INFINITY))) {
+      lo = min(lo, static_cast<int>(t));
+      hi = static_cast<int>(t) + 1;
+    }
+  }
+  atomicMin(&lo_s, lo);
+  atomicMax(&hi_s, hi);
+  __syncthreads();
+  if (threadIdx.x == 0)
+    rows.range[blockIdx.x] = hi_s > 0 ? make_int2(lo_s, hi_s) : make_int2(static_cast<int>(start), static_cast<int>(end));
+}
+
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
 
 struct Plan {
@@ -228,16 +258,41 @@ RowsChoice rows_choice(int64_t rows, int k_dim, int v_dim, int v_bits, int group
   return r;
 }
 
-// Rows times splits of any plan with at most these sequences, queries and tokens: n workgroups of k rows have at most
-// target / n splits, and at least one.
-int64_t most_partials(int B, int Hq, int L, int64_t max_tokens) {
-  const int64_t rows = rows_of(B, Hq, L), most = std::max<int64_t>(1, (max_tokens + kVecTokens - 1) / kVecTokens);
-  return std::min(rows * most, std::max(kVecTarget * kVecRows, kRaggedTarget * 16) + rows);
+// The many-rows kernel takes what the few-rows kernel does at its head dims, for more than one block of 16 rows, and
+// counts tokens in 32 bits.
+bool tile_kernel(int64_t rows, int k_dim, int v_dim, int64_t max_tokens) {
+  return rows > 16 && tile_rows(k_dim, v_dim) > 0 && max_tokens <= (1 << 30);
 }
 
-int64_t workspace_bytes(int B, int Hq, int L, int v_dim, int64_t max_tokens) {
-  const int64_t n = most_partials(B, Hq, L, max_tokens);
-  return align256(n * 8) + align256(n * v_dim * 4);
+constexpr int64_t kTileTarget = 256;  // workgroups at once: its eight waves fill a CU
+
+// Splits with the least estimated time: rounds of one workgroup a CU, each of its tokens and about 256 tokens' worth of
+// prologue and results; and the partial results' way through memory, 64 tokens' worth a round of 256 x 256 rows.
+Plan tile_plan(int64_t blocks, int64_t max_tokens) {
+  int64_t best = 1;
+  double best_time = 0;
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(1, 2 * kTileTarget / blocks), (max_tokens + 255) / 256);
+  for (int64_t s = 1; s <= std::max<int64_t>(1, most); ++s) {
+    const double rounds = static_cast<double>((blocks * s + kTileTarget - 1) / kTileTarget);
+    const double time = rounds * (static_cast<double>(max_tokens) / s + 256) +
+                        (s > 1 ? 128 + 128.0 * blocks * s / kTileTarget : 0);
+    if (s == 1 || time < best_time) best = s, best_time = time;
+  }
+  return {static_cast<int>(best), 0};  // the kernel divides the tokens that its rows see
+}
+
+// Rows times splits of any plan with at most these sequences, queries and tokens: n workgroups of k rows have at most
+// target / n splits, and at least one.
+int64_t most_partials(int B, int Hq, int Hkv, int L, int64_t max_tokens) {
+  const int64_t rows = rows_of(B, Hq, L), most = std::max<int64_t>(1, (max_tokens + kVecTokens - 1) / kVecTokens);
+  const int64_t few = std::max(kVecTarget * kVecRows, kRaggedTarget * 16);
+  const int64_t many = static_cast<int64_t>(Hq / Hkv) * L > 16 ? std::max(few, 2 * kTileTarget * 256) : few;
+  return std::min(rows * most, many + rows);
+}
+
+int64_t workspace_bytes(int B, int Hq, int Hkv, int L, int v_dim, int64_t max_tokens) {
+  const int64_t n = most_partials(B, Hq, Hkv, L, max_tokens);
+  return align256(n * 8) + align256(n * v_dim * 4) + align256(rows_of(B, Hq, L) * 8);
 }
 
 template <int DT>
@@ -268,7 +323,7 @@ int64_t tq_attention_affine_workspace_size(int B, int Hq, int Hkv, int L, int k_
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || L <= 0 || Hq % Hkv || max_tokens < 0 || k_dim <= 0 || v_dim <= 0 ||
       k_dim > kMaxDim || v_dim > kMaxDim)
     return 0;
-  return workspace_bytes(B, Hq, L, v_dim, max_tokens);
+  return workspace_bytes(B, Hq, Hkv, L, v_dim, max_tokens);
 }
 
 int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int L, int k_dim, int v_dim,
@@ -300,7 +355,7 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   if (B == 0 || Hq == 0 || L == 0) return TQ_OK;
   if (!q || !out || (max_tokens > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
     return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: null pointer");
-  const int64_t need = workspace_bytes(B, Hq, L, v_dim, max_tokens);
+  const int64_t need = workspace_bytes(B, Hq, Hkv, L, v_dim, max_tokens);
   if (!workspace || workspace_bytes_given < need)
     return fail(TQ_ERR_WORKSPACE, "tq_attention_affine: workspace of %lld bytes, %lld needed",
                 static_cast<long long>(workspace_bytes_given), static_cast<long long>(need));
@@ -311,11 +366,13 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
 
   const bool by_rows = rows_kernel(q_dtype, k_dim, v_dim, k_bits, v_bits);
   const RowsChoice rc = rows_choice(rows64, k_dim, v_dim, v_bits, group);
-  const int block_rows = by_rows ? rc.rows : kVecRows;
+  const bool by_tile = by_rows && tile_kernel(rows64, k_dim, v_dim, max_tokens);
+  const int block_rows = by_tile ? tile_rows(k_dim, v_dim) : by_rows ? rc.rows : kVecRows;
   const int64_t blocks1 = static_cast<int64_t>(B) * Hkv * ((rows64 + block_rows - 1) / block_rows);
   const bool ragged = seq_lens || seq_starts;
-  const Plan pl = by_rows ? plan_splits(blocks1, max_tokens, ragged ? kRaggedTarget : kRowsTarget, kRowsTokens)
-                          : plan_splits(blocks1, max_tokens, kVecTarget, kVecTokens);
+  const Plan pl = by_tile ? tile_plan(blocks1, max_tokens)
+                  : by_rows ? plan_splits(blocks1, max_tokens, ragged ? kRaggedTarget : kRowsTarget, kRowsTokens)
+                            : plan_splits(blocks1, max_tokens, kVecTarget, kVecTokens);
   AffineAttnParams p{};
   p.q = q;
   p.q_sb = q_stride_b, p.q_sh = q_stride_h, p.q_sl = q_stride_l;
@@ -340,7 +397,21 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned n_blocks = static_cast<unsigned>(blocks);
-  if (by_rows) {
+  if (by_tile) {
+    MaskRows mr{};
+    if (mask_kind != TQ_MASK_NONE) {
+      mr.range = reinterpret_cast<int2*>(static_cast<char*>(workspace) + align256(n * 8) + align256(n * v_dim * 4));
+      mr.nb = p.mask_s[0] || ragged ? B : 1;
+      mr.ng = p.mask_s[1] ? Hkv : 1;
+      mr.nr = p.mask_s[2] ? p.R : 1;
+      mr.nl = p.mask_s[3] || causal ? L : 1;
+      affine_mask_range_kernel<<<mr.nb * mr.ng * mr.nr * mr.nl, 256, 0, st>>>(p, mr);
+    }
+    const int rc_launch = k_bits == 4   ? launch_tile_k4v4(p, mr, q_dtype, st)
+                          : v_bits == 4 ? launch_tile_k8v4(p, mr, q_dtype, st)
+                                        : launch_tile_k8v8(p, mr, q_dtype, st);
+    if (rc_launch != TQ_OK || pl.splits == 1) return rc_launch;
+  } else if (by_rows) {
     const int rc_launch = k_bits == 4   ? launch_rows_k4v4(p, rc, q_dtype, st)
                           : v_bits == 4 ? launch_rows_k8v4(p, rc, q_dtype, st)
                                         : launch_rows_k8v8(p, rc, q_dtype, st);

@@ -90,13 +90,6 @@ __device__ __forceinline__ u32x4_t key_operand(const uint32_t* w) {
   return o;
 }
 
-// (scale, bias) of a packed pair of 16-bit values.
-template <int DT>
-__device__ __forceinline__ float2 pair_of(uint32_t u) {
-  if constexpr (DT == TQ_DTYPE_F16) return make_float2(f16_bits_to_f32(u & 0xffffu), f16_bits_to_f32(u >> 16));
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-
 template <int DT, int KB, int VB, int DP, int GS, int RPT, bool FULL>
 __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void affine_rows_kernel(const AffineAttnParams p) {
   using S = RowsShape<KB, VB, DP, GS, RPT>;
@@ -135,7 +128,7 @@ __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void 
         const uint32_t w[4] = {raw[g][ch].x, raw[g][ch].y, raw[g][ch].z, raw[g][ch].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 t = pair_of<DT>(w[j]);
+          const float2 t = pair16<DT>(w[j]);
           big = fmaxf(big, fmaxf(fabsf(t.x), fabsf(t.y)));
         }
       }
@@ -154,7 +147,7 @@ __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void 
         _Float16 f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 t = pair_of<DT>(w[j]);
+          const float2 t = pair16<DT>(w[j]);
           f[2 * j] = static_cast<_Float16>(t.x * scale_up), f[2 * j + 1] = static_cast<_Float16>(t.y * scale_up);
         }
 #pragma unroll
@@ -321,7 +314,7 @@ __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void 
         float s = 0.f;
 #pragma unroll
         for (int g = 0; g < S::NG; ++g) {
-          const float2 sb = pair_of<DT>(kp[u][j][g]);
+          const float2 sb = pair16<DT>(kp[u][j][g]);
           s = __builtin_fmaf(sb.x, dot[g][j], __builtin_fmaf(sb.y, qsum[g], s));
         }
         s *= row_scale;
@@ -377,7 +370,7 @@ __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void 
           float v[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 sb = pair_of<DT>(vp[u][j][s][a]);
+            const float2 sb = pair16<DT>(vp[u][j][s][a]);
             // what a row masks may be NaN
             v[j] = w[j] == 0.f ? 0.f : w[j] * sb.x;
             corr[s][a] = w[j] == 0.f ? corr[s][a] : __builtin_fmaf(w[j], sb.y, corr[s][a]);

@@ -1,0 +1,478 @@
+// Attention of many query rows (prefill chunks) over the group-affine cache, on the matrix cores.
+//
+// A workgroup takes 8 waves x RT x 16 query rows of one kv head.  Every 64 tokens it decodes keys and values into LDS
+// once for all of them, as the vectors' own type (scale * code + bias in f32, rounded once: an error of half a step a
+// coordinate, as the reference's layers have it, which dequantize in that type), half the waves the keys and half the
+// values, while the tile before is worked on:
+//   scores  C[token][row] = K Q^T (v_mfma_f32_16x16x32), keys row by row in LDS, queries in registers.
+//   values  O[row][coordinate] = P V: C's lanes hold row = lane % 16 and tokens 4 (lane / 16) + j of every 16-token
+//           tile, which is A's layout when 32 tokens are taken in the order (lane / 16, tile, j); values lie in LDS
+//           transposed and in that order, so weights go from C to A in registers, and the sum of a row's rounded
+//           weights is one more product with ones.
+// Softmax: one reference a row, moved only when a score passes it by 8 (base 2).  Weights go in as one 16-bit number
+// (bf16: 2^-8 of the weight at most; f16: truncated, 2^-10, and up to 2^15 so that small ones stay normal); they are
+// divided by the sum of the same rounded numbers.
+//
+// A token whose values are not finite has zeros in LDS and a flag; the rows that weigh it add it on the vector units,
+// so what a row masks may be NaN.  A group that would leave its type's range when rounded is cut to it.
+//
+// What bounds it, d = 128, a step of 64 tokens and 256 rows a CU: matrix products 2048 cycles, LDS reads 2048, vector
+// instructions about 2400 a SIMD (softmax 7 a score, decoding 3 an element).
+#pragma once
+
+#include "tq_affine.h"
+#include "tq_pieces.h"
+
+namespace tq {
+
+constexpr int kTileWaves = 8;
+constexpr int kTileStep = 64;  // tokens in LDS at a time
+
+template <int KS, int CT>
+struct TileShape {
+  static constexpr int DK = 32 * KS, DV = 16 * CT;
+  static constexpr int RT = KS <= 4 && CT <= 8 ? 2 : 1;  // 16-row tiles a wave
+  static constexpr int ROWS = kTileWaves * 16 * RT;
+  static constexpr int KROW = DK + 8;          // 16-bit elements of a token's row of keys in LDS
+  static constexpr int VROW = kTileStep + 8;   // of a coordinate's row of values
+  static constexpr int KBUF = kTileStep * KROW, VBUF = DV * VROW;
+  static constexpr int KU = KS;                // 8-coordinate pieces of keys a decoding thread has (256 threads)
+  static constexpr int VU = (CT + 7) / 8;      // (4 tokens x 8 coordinates) units of values
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma_of(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (DT == TQ_DTYPE_BF16) return mfma_bf16(a, b, c);
+  typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                0);
+}
+
+// Two f32 as 16-bit numbers, to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pack_of(float lo, float hi) {
+  if constexpr (DT == TQ_DTYPE_BF16) {
+    const bf16x2_t t = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, t);
+  } else {
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    const f16x2_t t = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, t);
+  }
+}
+
+// Eight codes as f32: one word of 4-bit codes or two of 8-bit ones.
+template <int BITS>
+__device__ __forceinline__ void codes_f32(const uint32_t* w, float (&f)[8]) {
+  if constexpr (BITS == 4) {
+    const uint32_t even = w[0] & 0x0f0f0f0fu, odd = (w[0] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[2 * j] = static_cast<float>((even >> (8 * j)) & 0xffu);
+      f[2 * j + 1] = static_cast<float>((odd >> (8 * j)) & 0xffu);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = static_cast<float>((w[j >> 2] >> (8 * (j & 3))) & 0xffu);
+  }
+}
+
+// Whether every value scale * code + bias rounds to a finite number of the type.
+template <int DT, int BITS>
+__device__ __forceinline__ bool in_range(float2 sb) {
+  const float most = DT == TQ_DTYPE_F16 ? 65504.f : 0x1.fep127f;
+  return fabsf(sb.y) + static_cast<float>((1 << BITS) - 1) * fabsf(sb.x) <= most;  // false for NaN
+}
+
+// A value cut to the type's range; NaN and infinite pairs give zeros (the flagged way adds them).
+template <int DT>
+__device__ __forceinline__ float cut(float2 sb, float code) {
+  const float most = DT == TQ_DTYPE_F16 ? 65504.f : 0x1.fep127f;
+  if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY)) return 0.f;
+  return fminf(fmaxf(__builtin_fmaf(sb.x, code, sb.y), -most), most);
+}
+
+template <int DT, int KB, int VB, int KS, int CT>
+__global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const AffineAttnParams p, const MaskRows mrows) {
+  using S = TileShape<KS, CT>;
+  constexpr int RT = S::RT;
+  __shared__ __attribute__((aligned(16))) uint16_t k_lds[2][S::KBUF];
+  __shared__ __attribute__((aligned(16))) uint16_t v_lds[2][S::VBUF];
+  __shared__ uint32_t bad_lds[3][2];  // tokens whose values are not finite, of three steps
+  __shared__ int range_lds[2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, q4 = lane >> 4;
+  const int row_blocks = (p.rows + S::ROWS - 1) / S::ROWS;
+  const int split = blockIdx.x % p.splits;
+  const int blk = blockIdx.x / p.splits;
+  const int bh = blk / row_blocks, block_row0 = (blk % row_blocks) * S::ROWS;
+  const int b = bh / p.Hkv, h = bh % p.Hkv;
+  const int row0 = block_row0 + wave * 16 * RT;
+
+  int64_t start, end;
+  affine_range(p, b, start, end);
+
+  // tokens that any row of this workgroup sees
+  int first = static_cast<int>(start), stop = static_cast<int>(end);
+  if (p.mask_kind != TQ_MASK_NONE) {
+    if (tid == 0) range_lds[0] = stop, range_lds[1] = first;
+    __syncthreads();
+    int lo = stop, hi = first;
+    for (int i = tid; i < S::ROWS; i += 64 * kTileWaves) {
+      const int row = min(block_row0 + i, p.rows - 1);
+      const int l = row / p.R, r = row % p.R;
+      const int64_t at = ((static_cast<int64_t>(mrows.nb > 1 ? b : 0) * mrows.ng + (mrows.ng > 1 ? h : 0)) * mrows.nr +
+                          (mrows.nr > 1 ? r : 0)) * mrows.nl + (mrows.nl > 1 ? l : 0);
+      const int2 t = mrows.range[at];
+      lo = min(lo, t.x), hi = max(hi, t.y);
+    }
+    atomicMin(&range_lds[0], lo);
+    atomicMax(&range_lds[1], hi);
+    __syncthreads();
+    first = range_lds[0], stop = range_lds[1];
+  } else if (p.causal) {
+    const int l_lo = block_row0 / p.R, l_hi = (min(block_row0 + S::ROWS, p.rows) - 1) / p.R;
+    if (end - p.L + l_lo >= start) stop = static_cast<int>(end - p.L + l_hi + 1);
+  }
+  const int per = ((stop - first + p.splits - 1) / p.splits + kTileStep - 1) / kTileStep * kTileStep;
+  const int t0 = first + min(static_cast<int64_t>(split) * per, static_cast<int64_t>(stop - first));
+  const int t1 = min(stop, t0 + per);
+
+  // this lane's query rows, as columns of C
+  u32x4_t qop[RT][KS];
+  int lim[RT];
+  int64_t mask_at[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = min(row0 + rt * 16 + c, p.rows - 1);
+    const int l = row / p.R, r = row % p.R;
+    const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + (static_cast<int64_t>(h) * p.R + r) * p.q_sh +
+                        static_cast<int64_t>(l) * p.q_sl;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const uint4 u = *reinterpret_cast<const uint4*>(q + s * 32 + q4 * 8);
+      qop[rt][s] = u32x4_t{u.x, u.y, u.z, u.w};
+      // a negative scale turns the queries' signs, so that the largest product has the largest score
+      if (p.scale < 0.f) qop[rt][s] ^= u32x4_t{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    }
+    lim[rt] = p.causal ? static_cast<int>(end) - p.L + l : INT32_MAX;
+    mask_at[rt] = p.mask_kind != TQ_MASK_NONE
+                      ? b * p.mask_s[0] + h * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3] : 0;
+  }
+  const float scale = fabsf(p.scale);
+  // the causal rule leaves a step of tokens alone when its last one is within the first row's limit
+  const int lim_min = p.causal ? static_cast<int>(end) - p.L + row0 / p.R : INT32_MAX;
+
+  float m[RT], ref[RT];
+  f32x4_t acc[RT][CT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY, ref[rt] = 0.f;
+    sum[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < CT; ++n) acc[rt][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ---- decoding: waves 0..3 keys, 4..7 values
+  const bool keys = wave < kTileWaves / 2;
+  const int dtid = tid & 255;
+  const int64_t base = static_cast<int64_t>(bh) * p.capacity;
+  const int shift = p.group == 32 ? 2 : p.group == 64 ? 3 : 4;  // 8-coordinate pieces a group
+  constexpr int KWORDS = KB / 4, VWORDS = VB / 4;
+  constexpr int KREGS = S::KU * (KWORDS + 1), VREGS = S::VU * 4 * (VWORDS + 1);
+  uint32_t raw[KREGS > VREGS ? KREGS : VREGS];
+
+  auto load = [&](int t) {
+    const int last = min(t1 - t, kTileStep) - 1;
+    if (keys) {
+      const uint32_t* codes = p.k_codes + (base + t) * (S::DK * KB / 32);
+      const uint32_t* pairs = static_cast<const uint32_t*>(p.k_params) + (base + t) * (S::DK >> (shift + 3));
+#pragma unroll
+      for (int i = 0; i < S::KU; ++i) {
+        const uint32_t unit = i * 256 + dtid;
+        const uint32_t tok = min(static_cast<int>(unit / (KS * 4)), last), piece = unit % (KS * 4);
+        const uint32_t at = tok * (S::DK * KB / 32) + piece * KWORDS;
+        if constexpr (KWORDS == 1) {
+          raw[i * 2] = codes[at];
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(codes + at);
+          raw[i * 3] = u.x, raw[i * 3 + 1] = u.y;
+        }
+        raw[i * (KWORDS + 1) + KWORDS] = pairs[tok * (S::DK >> (shift + 3)) + (piece >> shift)];
+      }
+    } else {
+      const uint32_t* codes = p.v_codes + (base + t) * (S::DV * VB / 32);
+      const uint32_t* pairs = static_cast<const uint32_t*>(p.v_params) + (base + t) * (S::DV >> (shift + 3));
+#pragma unroll
+      for (int i = 0; i < S::VU; ++i) {
+        const uint32_t unit = i * 256 + dtid;
+        const uint32_t quad = unit % 16, piece = min(unit / 16, static_cast<uint32_t>(CT * 2 - 1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t tok = min(static_cast<int>(quad * 4 + j), last);
+          const uint32_t at = tok * (S::DV * VB / 32) + piece * VWORDS;
+          uint32_t* to = raw + (i * 4 + j) * (VWORDS + 1);
+          if constexpr (VWORDS == 1) {
+            to[0] = codes[at];
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(codes + at);
+            to[0] = u.x, to[1] = u.y;
+          }
+          to[VWORDS] = pairs[tok * (S::DV >> (shift + 3)) + (piece >> shift)];
+        }
+      }
+    }
+  };
+
+  auto decode = [&](int buf, int flags) {
+    if (keys) {
+#pragma unroll
+      for (int i = 0; i < S::KU; ++i) {
+        const uint32_t unit = i * 256 + dtid;
+        const uint32_t tok = unit / (KS * 4), piece = unit % (KS * 4);
+        const uint32_t* w = raw + i * (KWORDS + 1);
+        const float2 sb = pair16<DT>(w[KWORDS]);
+        float f[8];
+        codes_f32<KB>(w, f);
+        u32x4_t o;
+        if (in_range<DT, KB>(sb)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = pack_of<DT>(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y));
+        } else {  // NaN stays
+          const bool nan = !(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = nan ? pack_of<DT>(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y))
+                       : pack_of<DT>(cut<DT>(sb, f[2 * j]), cut<DT>(sb, f[2 * j + 1]));
+        }
+        *reinterpret_cast<u32x4_t*>(&k_lds[buf][tok * S::KROW + piece * 8]) = o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::VU; ++i) {
+        const uint32_t unit = i * 256 + dtid;
+        const uint32_t quad = unit % 16, piece = unit / 16;
+        if (piece >= CT * 2) break;
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t* w = raw + (i * 4 + j) * (VWORDS + 1);
+          const float2 sb = pair16<DT>(w[VWORDS]);
+          codes_f32<VB>(w, v[j]);
+          if (in_range<DT, VB>(sb)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = __builtin_fmaf(sb.x, v[j][e], sb.y);
+          } else {
+            if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY))
+              atomicOr(&bad_lds[flags][quad >> 3], 1u << ((quad * 4 + j) & 31));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = cut<DT>(sb, v[j][e]);
+          }
+        }
+        // tokens 4 quad + j: 32 (quad / 8) + 8 (quad % 4) + 4 (quad / 4 % 2) + j in the order of A's k indices
+        const uint32_t pos = (quad >> 3) * 32 + (quad & 3) * 8 + ((quad >> 2) & 1) * 4;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint2 two = make_uint2(pack_of<DT>(v[0][e], v[1][e]), pack_of<DT>(v[2][e], v[3][e]));
+          *reinterpret_cast<uint2*>(&v_lds[buf][(piece * 8 + e) * S::VROW + pos]) = two;
+        }
+      }
+    }
+  };
+
+  if (tid < 6) bad_lds[tid >> 1][tid & 1] = 0;
+  __syncthreads();
+  if (t0 < t1) {
+    load(t0);
+    decode(0, 0);
+    if (t0 + kTileStep < t1) load(t0 + kTileStep);
+  }
+  __syncthreads();
+
+  int buf = 0, flags = 0;  // flags: a step's, the next's (written now) and the one after (cleared now)
+  for (int t = t0; t < t1; t += kTileStep, buf ^= 1, flags = flags == 2 ? 0 : flags + 1) {
+    const bool more = t + kTileStep < t1;
+    // ---- scores
+    f32x4_t C[RT][4];
+#pragma unroll
+    for (int ti = 0; ti < 4; ++ti) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) C[rt][ti] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const u32x4_t k = *reinterpret_cast<const u32x4_t*>(&k_lds[buf][(ti * 16 + c) * S::KROW + s * 32 + q4 * 8]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) C[rt][ti] = mfma_of<DT>(k, qop[rt][s], C[rt][ti]);
+      }
+    }
+    // the next tile into the other half of LDS, and its successor's codes on their way
+    if (tid < 2) bad_lds[flags == 0 ? 2 : flags - 1][tid] = 0;
+    if (more) {
+      decode(buf ^ 1, flags == 2 ? 0 : flags + 1);
+      if (t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
+    }
+
+    // ---- softmax
+    const bool plain = p.mask_kind == TQ_MASK_NONE && t + kTileStep - 1 <= lim_min && t + kTileStep <= t1;
+    u32x4_t A[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float top;
+      if (plain) {
+        top = C[rt][0][0];
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, C[rt][ti][j]);
+        top *= scale;
+      } else {
+        top = -INFINITY;
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y = C[rt][ti][j] * scale;
+            const int tok = t + ti * 16 + q4 * 4 + j;
+            if (p.mask_kind != TQ_MASK_NONE) y = affine_mask(p, mask_at[rt] + min(tok, t1 - 1) * p.mask_s[4], y);
+            if (tok > lim[rt] && y != -INFINITY) y = -FLT_MAX;
+            if (tok >= t1) y = -INFINITY;
+            C[rt][ti][j] = y;
+            top = fmaxf(top, y);
+          }
+      }
+      if (__any(top > m[rt] + 8.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = fmaxf(m[rt], top);
+        // f16 weights reach 2^(8 + 7)
+        const float ref_to = to == -INFINITY ? 0.f : DT == TQ_DTYPE_F16 ? to - 7.f : to;
+        const float a = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[rt] - ref_to);
+        m[rt] = to, ref[rt] = ref_to;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float aj = __shfl(a, q4 * 4 + j);
+          sum[rt][j] *= aj;
+#pragma unroll
+          for (int n = 0; n < CT; ++n) acc[rt][n][j] *= aj;
+        }
+      }
+      if (plain) {
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) C[rt][ti][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(C[rt][ti][j], scale, -ref[rt]));
+      } else {
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) C[rt][ti][j] = __builtin_amdgcn_exp2f(C[rt][ti][j] - ref[rt]);
+      }
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lo = C[rt][2 * pr + j / 2][2 * (j & 1)], hi = C[rt][2 * pr + j / 2][2 * (j & 1) + 1];
+          if constexpr (DT == TQ_DTYPE_BF16)
+            A[rt][pr][j] = pack_of<DT>(lo, hi);
+          else
+            A[rt][pr][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+        }
+    }
+
+    // ---- values
+    constexpr uint32_t kOnes = DT == TQ_DTYPE_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    const u32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma_of<DT>(A[rt][pr], ones, sum[rt]);
+#pragma unroll
+      for (int n = 0; n < CT; ++n) {
+        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(&v_lds[buf][(n * 16 + c) * S::VROW + pr * 32 + q4 * 8]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][n] = mfma_of<DT>(A[rt][pr], v, acc[rt][n]);
+      }
+    }
+
+    // ---- tokens whose values are not finite, for the rows that weigh them
+    const uint32_t bad0 = __builtin_amdgcn_readfirstlane(bad_lds[flags][0]), bad1 = __builtin_amdgcn_readfirstlane(bad_lds[flags][1]);
+    if (bad0 | bad1) {
+#pragma unroll 1
+      for (int tok = 0; tok < kTileStep; ++tok) {
+        if (!(((tok < 32 ? bad0 : bad1) >> (tok & 31)) & 1u) || t + tok >= t1) continue;
+        const int64_t at = base + t + tok;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float w = 0.f;
+#pragma unroll
+          for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w = tok / 16 == ti && tok % 4 == j ? C[rt][ti][j] : w;
+          float wr[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wr[j] = __shfl(w, (tok % 16) / 4 * 16 + q4 * 4 + j);
+#pragma unroll
+          for (int n = 0; n < CT; ++n) {
+            const int d = n * 16 + c;
+            const float2 sb = pair16<DT>(static_cast<const uint32_t*>(p.v_params)[at * (S::DV >> (shift + 3)) + (d >> (shift + 3))]);
+            if ((fabsf(sb.x) < INFINITY) && (fabsf(sb.y) < INFINITY)) continue;  // in LDS already
+            const uint32_t word = p.v_codes[at * (S::DV * VB / 32) + d * VB / 32];
+            const float v = __builtin_fmaf(sb.x, static_cast<float>((word >> (d * VB % 32)) & ((1u << VB) - 1u)), sb.y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[rt][n][j] = wr[j] == 0.f ? acc[rt][n][j] : __builtin_fmaf(wr[j], v, acc[rt][n][j]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // ---- results: rows 4 q4 + j, coordinates 16 n + c
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + rt * 16 + q4 * 4 + j;
+      const float row_ref = __shfl(m[rt] == -INFINITY ? -INFINITY : ref[rt], q4 * 4 + j);
+      if (row >= p.rows) continue;
+      const float l = sum[rt][j];
+      if (p.splits == 1) {
+        const int64_t head = static_cast<int64_t>(bh) * p.R + row % p.R;
+        const int64_t to = (head * p.L + row / p.R) * S::DV + c;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int n = 0; n < CT; ++n) store_elem<DT>(p.out, to + n * 16, l == 0.f ? 0.f : acc[rt][n][j] * inv);
+      } else {
+        const int64_t at = (static_cast<int64_t>(bh) * p.rows + row) * p.splits + split;
+#pragma unroll
+        for (int n = 0; n < CT; ++n) p.part_o[at * S::DV + n * 16 + c] = acc[rt][n][j];
+        if (c == 0) p.part_ml[2 * at] = row_ref, p.part_ml[2 * at + 1] = l;
+      }
+    }
+}
+
+template <int DT, int KB, int VB, int KS, int CT>
+int launch_tile_at(const AffineAttnParams& p, const MaskRows& m, hipStream_t st) {
+  constexpr int kRows = TileShape<KS, CT>::ROWS;
+  static_assert(kRows == tile_rows(32 * KS, 16 * CT), "rows a workgroup");
+  const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * ((p.rows + kRows - 1) / kRows) * p.splits;
+  if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
+  affine_tile_kernel<DT, KB, VB, KS, CT><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
+  return check_launch("affine_tile_kernel");
+}
+
+template <int DT, int KB, int VB>
+int launch_tile_bits(const AffineAttnParams& p, const MaskRows& m, hipStream_t st) {
+  switch (p.k_dim) {
+    case 64: return launch_tile_at<DT, KB, VB, 2, 4>(p, m, st);
+    case 96: return launch_tile_at<DT, KB, VB, 3, 6>(p, m, st);
+    case 128: return launch_tile_at<DT, KB, VB, 4, 8>(p, m, st);
+    case 192: return launch_tile_at<DT, KB, VB, 6, 8>(p, m, st);
+    case 256: return launch_tile_at<DT, KB, VB, 8, 16>(p, m, st);
+    default: return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: no tile kernel for head dims %d / %d", p.k_dim, p.v_dim);
+  }
+}
+
+}  // namespace tq

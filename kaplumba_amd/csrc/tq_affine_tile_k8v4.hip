@@ -1,0 +1,11 @@
+// The many-rows kernel over 8-bit keys and 4-bit values.
+#include "tq_affine_tile.h"
+
+namespace tq {
+
+int launch_tile_k8v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st) {
+  return dtype == TQ_DTYPE_F16 ? launch_tile_bits<TQ_DTYPE_F16, 8, 4>(p, m, st)
+                               : launch_tile_bits<TQ_DTYPE_BF16, 8, 4>(p, m, st);
+}
+
+}  // namespace tq
