@@ -35,8 +35,9 @@ struct AffineAttnParams {
   float* part_ml;         // [B * Hkv * rows, splits, 2]: running maximum (base 2), sum
 };
 
-// Which instantiation of the few-rows kernel (tq_affine_rows.h) takes a call: head dims up to `dim`, exactly it
-// where `full`, and `rows` query rows a workgroup.
+// Which instantiation of the few-rows kernel (tq_affine_rows.h) takes a call: head dims up to `dim`, exactly it and no
+// array mask where `full`, and `rows` query rows a workgroup.  (The mask's loads, between the codes' and their use, would
+// make every call wait for the next step's codes.)
 struct RowsChoice {
   int dim, rows;
   bool full;
@@ -67,8 +68,9 @@ int launch_tile_k8v8(const AffineAttnParams& p, const MaskRows& m, int dtype, hi
 
 // Tokens [start, end) of sequence b, as the device arrays say, within the cache.
 __device__ __forceinline__ void affine_range(const AffineAttnParams& p, int b, int64_t& start, int64_t& end) {
-  end = p.lens ? min(static_cast<int64_t>(p.lens[b]), p.max_tokens) : p.max_tokens;
-  start = p.starts ? max(static_cast<int64_t>(p.starts[b]), static_cast<int64_t>(0)) : 0;
+  // uniform: b is the workgroup's
+  end = p.lens ? min(static_cast<int64_t>(__builtin_amdgcn_readfirstlane(p.lens[b])), p.max_tokens) : p.max_tokens;
+  start = p.starts ? max(static_cast<int64_t>(__builtin_amdgcn_readfirstlane(p.starts[b])), static_cast<int64_t>(0)) : 0;
   if (end < start) end = start;
 }
 
@@ -82,6 +84,28 @@ __device__ __forceinline__ float affine_mask(const AffineAttnParams& p, int64_t 
   if (m == -INFINITY) return m;  // also where the score is not finite
   const float t = __builtin_fmaf(m, 1.44269504088896341f, x);
   return t == -INFINITY ? -FLT_MAX : t;
+}
+
+// A load at a uniform base and a lane's offset in bytes, in 32 bits: the form that global loads have for it (an index
+// of words would first be widened and added on the vector units).
+template <typename T>
+__device__ __forceinline__ T load_at(const void* base, uint32_t bytes) {
+  return *reinterpret_cast<const T*>(static_cast<const char*>(base) + bytes);
+}
+
+// A constant that the compiler holds in a register.  Neither operand of (x & mask) | with fits v_and_or_b32 as a
+// literal, so it takes two instructions for constants it knows.  Only vector instructions may read the result of the
+// asm: the wait states between a vector write and a matrix instruction's read are the compiler's to insert, and it
+// does not look into asm.
+__device__ __forceinline__ uint32_t held_vector(uint32_t x) {
+  uint32_t o;
+  asm("v_mov_b32 %0, %1" : "=v"(o) : "s"(x));
+  return o;
+}
+__device__ __forceinline__ uint32_t held_scalar(uint32_t x) {
+  uint32_t o;
+  asm("s_mov_b32 %0, %1" : "=s"(o) : "i"(x));
+  return o;
 }
 
 // (scale, bias) of a packed pair of 16-bit values.

@@ -232,7 +232,7 @@ struct Plan {
 
 constexpr int64_t kVecTarget = 512;     // workgroups of the vector kernel to aim at: two a CU
 constexpr int64_t kRowsTarget = 256;    // of the few-rows kernel: eight waves, two a SIMD, on every CU
-constexpr int64_t kRaggedTarget = 1024; // where sequences end at different tokens: finer, so that CUs share the long ones
+constexpr int64_t kRaggedTarget = 768;  // where sequences end at different tokens: finer, so that CUs share the long ones
 constexpr int kRowsTokens = 512;        // tokens of one step of a workgroup's eight waves
 
 // A split for every `unit` tokens at most, and about `target` workgroups in all.
@@ -245,23 +245,23 @@ Plan plan_splits(int64_t blocks, int64_t max_tokens, int64_t target, int unit) {
 
 int64_t rows_of(int B, int Hq, int L) { return static_cast<int64_t>(B) * Hq * L; }
 
-// The few-rows kernel takes 16-bit types and head dims to 256 (f32 and larger dims: the vector kernel).
-bool rows_kernel(int dtype, int k_dim, int v_dim, int k_bits, int v_bits) {
-  return dtype != TQ_DTYPE_F32 && k_dim <= 256 && v_dim <= 256 && !(k_bits == 4 && v_bits == 8);
+// The few-rows kernel takes 16-bit types and head dims to 256 and counts tokens in 32 bits (f32, larger dims, 4-bit keys
+// with 8-bit values: the vector kernel).
+bool rows_kernel(int dtype, int k_dim, int v_dim, int k_bits, int v_bits, int64_t max_tokens) {
+  return max_tokens <= (1 << 30) && dtype != TQ_DTYPE_F32 && k_dim <= 256 && v_dim <= 256 && !(k_bits == 4 && v_bits == 8);
 }
 
-RowsChoice rows_choice(int64_t rows, int k_dim, int v_dim, int v_bits, int group) {
+RowsChoice rows_choice(int64_t rows, int k_dim, int v_dim, int group, int mask_kind) {
   RowsChoice r;
-  r.full = k_dim == v_dim && (k_dim == 64 || k_dim == 128 || k_dim == 256) && group <= 64;
+  r.full = k_dim == v_dim && (k_dim == 64 || k_dim == 128 || k_dim == 256) && group <= 64 && mask_kind == TQ_MASK_NONE;
   r.dim = r.full ? k_dim : std::max(k_dim, v_dim) <= 128 ? 128 : 256;
-  r.rows = r.full && rows <= 4 ? 4 : rows_large(v_bits, r.dim, group);
+  r.rows = r.full && rows <= 4 ? 4 : rows_large(r.dim, group);
   return r;
 }
 
-// The many-rows kernel takes what the few-rows kernel does at its head dims, for more than one block of 16 rows, and
-// counts tokens in 32 bits.
-bool tile_kernel(int64_t rows, int k_dim, int v_dim, int64_t max_tokens) {
-  return rows > 16 && tile_rows(k_dim, v_dim) > 0 && max_tokens <= (1 << 30);
+// The many-rows kernel takes what the few-rows kernel does at its head dims, for more than one block of 16 rows.
+bool tile_kernel(int64_t rows, int k_dim, int v_dim) {
+  return rows > 16 && tile_rows(k_dim, v_dim) > 0;
 }
 
 constexpr int64_t kTileTarget = 256;  // workgroups at once: its eight waves fill a CU
@@ -364,9 +364,9 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
        static_cast<uintptr_t>((q_stride_b | q_stride_h | q_stride_l) * (q_dtype == TQ_DTYPE_F32 ? 4 : 2))) & 15)
     return fail(TQ_ERR_INVALID_ARGUMENT, "tq_attention_affine: queries, their strides and the codes must be 16-byte aligned");
 
-  const bool by_rows = rows_kernel(q_dtype, k_dim, v_dim, k_bits, v_bits);
-  const RowsChoice rc = rows_choice(rows64, k_dim, v_dim, v_bits, group);
-  const bool by_tile = by_rows && tile_kernel(rows64, k_dim, v_dim, max_tokens);
+  const bool by_rows = rows_kernel(q_dtype, k_dim, v_dim, k_bits, v_bits, max_tokens);
+  const RowsChoice rc = rows_choice(rows64, k_dim, v_dim, group, mask_kind);
+  const bool by_tile = by_rows && tile_kernel(rows64, k_dim, v_dim);
   const int block_rows = by_tile ? tile_rows(k_dim, v_dim) : by_rows ? rc.rows : kVecRows;
   const int64_t blocks1 = static_cast<int64_t>(B) * Hkv * ((rows64 + block_rows - 1) / block_rows);
   const bool ragged = seq_lens || seq_starts;

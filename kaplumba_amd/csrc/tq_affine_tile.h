@@ -192,14 +192,14 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
       for (int i = 0; i < S::KU; ++i) {
         const uint32_t unit = i * 256 + dtid;
         const uint32_t tok = min(static_cast<int>(unit / (KS * 4)), last), piece = unit % (KS * 4);
-        const uint32_t at = tok * (S::DK * KB / 32) + piece * KWORDS;
+        const uint32_t at = (tok * (S::DK * KB / 32) + piece * KWORDS) * 4;
         if constexpr (KWORDS == 1) {
-          raw[i * 2] = codes[at];
+          raw[i * 2] = load_at<uint32_t>(codes, at);
         } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(codes + at);
+          const uint2 u = load_at<uint2>(codes, at);
           raw[i * 3] = u.x, raw[i * 3 + 1] = u.y;
         }
-        raw[i * (KWORDS + 1) + KWORDS] = pairs[tok * (S::DK >> (shift + 3)) + (piece >> shift)];
+        raw[i * (KWORDS + 1) + KWORDS] = load_at<uint32_t>(pairs, (tok * (S::DK >> (shift + 3)) + (piece >> shift)) * 4);
       }
     } else {
       const uint32_t* codes = p.v_codes + (base + t) * (S::DV * VB / 32);
@@ -211,15 +211,15 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t tok = min(static_cast<int>(quad * 4 + j), last);
-          const uint32_t at = tok * (S::DV * VB / 32) + piece * VWORDS;
+          const uint32_t at = (tok * (S::DV * VB / 32) + piece * VWORDS) * 4;
           uint32_t* to = raw + (i * 4 + j) * (VWORDS + 1);
           if constexpr (VWORDS == 1) {
-            to[0] = codes[at];
+            to[0] = load_at<uint32_t>(codes, at);
           } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(codes + at);
+            const uint2 u = load_at<uint2>(codes, at);
             to[0] = u.x, to[1] = u.y;
           }
-          to[VWORDS] = pairs[tok * (S::DV >> (shift + 3)) + (piece >> shift)];
+          to[VWORDS] = load_at<uint32_t>(pairs, (tok * (S::DV >> (shift + 3)) + (piece >> shift)) * 4);
         }
       }
     }
