@@ -193,6 +193,51 @@ __global__ __launch_bounds__(256) void affine_merge_kernel(const AffineAttnParam
   }
 }
 
+// The same for few splits: a thread takes four coordinates of a row over all of them, so that prefill's many rows
+// are one stream of the partial results.
+template <int DT>
+__global__ __launch_bounds__(256) void affine_merge_flat_kernel(const AffineAttnParams p, uint32_t quads, uint32_t all) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  const uint32_t at = i / quads;  // (b, h, row)
+  const uint32_t d = (i - at * quads) * 4;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + static_cast<int64_t>(at) * p.splits;
+  const float* from = p.part_o + static_cast<int64_t>(at) * p.splits * p.v_dim + d;
+  float M = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, ml[s].x);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float4 o = {};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 t = ml[s];
+    const float4 x = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * p.v_dim);
+    const float w = __builtin_amdgcn_exp2f(t.x - ref);
+    sum = __builtin_fmaf(w, t.y, sum);
+    o.x = w == 0.f ? o.x : __builtin_fmaf(w, x.x, o.x), o.y = w == 0.f ? o.y : __builtin_fmaf(w, x.y, o.y);
+    o.z = w == 0.f ? o.z : __builtin_fmaf(w, x.z, o.z), o.w = w == 0.f ? o.w : __builtin_fmaf(w, x.w, o.w);
+  }
+  const uint32_t row = at % p.rows;
+  const int64_t bh = at / p.rows;
+  const int64_t to = ((bh * p.R + row % p.R) * p.L + row / p.R) * p.v_dim + d;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  store_elem<DT>(p.out, to, sum == 0.f ? 0.f : o.x * inv);
+  store_elem<DT>(p.out, to + 1, sum == 0.f ? 0.f : o.y * inv);
+  store_elem<DT>(p.out, to + 2, sum == 0.f ? 0.f : o.z * inv);
+  store_elem<DT>(p.out, to + 3, sum == 0.f ? 0.f : o.w * inv);
+}
+
+template <int DT>
+void launch_merge(const AffineAttnParams& p, int64_t rows, hipStream_t st) {
+  const int64_t quads = rows * (p.v_dim / 4);
+  // a row a workgroup hides the splits' latency where there are many of them and few rows
+  if (p.splits <= 16 && quads >= 65536 && quads <= INT32_MAX)
+    affine_merge_flat_kernel<DT><<<static_cast<unsigned>((quads + 255) / 256), 256, 0, st>>>(
+        p, static_cast<uint32_t>(p.v_dim / 4), static_cast<uint32_t>(quads));
+  else
+    affine_merge_kernel<DT><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
+}
+
 // One workgroup a row of MaskRows.
 __global__ __launch_bounds__(256) void affine_mask_range_kernel(const AffineAttnParams p, const MaskRows rows) {
   __shared__ int lo_s, hi_s;
@@ -209,13 +254,27 @@ __global__ __launch_bounds__(256) void affine_mask_range_kernel(const AffineAttn
   __syncthreads();
   const int64_t from = b * p.mask_s[0] + g * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3];
   int lo = INT32_MAX, hi = 0;
-  for (int64_t t = start + threadIdx.x; t < seen; t += 256) {
-    // a NaN counts as kept
-    if (!(affine_mask(p, from + t * p.mask_s[4], 0.f) <= (p.mask_kind == TQ_MASK_BOOL ? -FLT_MAX : -INFINITY))) {
-      lo = min(lo, static_cast<int>(t));
-      hi = static_cast<int>(t) + 1;
+  auto see = [&](int64_t t, bool kept) {
+    if (kept) lo = min(lo, static_cast<int>(t)), hi = max(hi, static_cast<int>(t) + 1);
+  };
+  // a NaN counts as kept
+  auto kept = [&](int64_t t) {
+    return !(affine_mask(p, from + t * p.mask_s[4], 0.f) <= (p.mask_kind == TQ_MASK_BOOL ? -FLT_MAX : -INFINITY));
+  };
+  int64_t t0 = start;
+  if (p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1) {  // eight bytes a thread where the row is contiguous
+    const uint8_t* m = static_cast<const uint8_t*>(p.mask) + from;
+    for (; t0 + 2048 <= seen; t0 += 2048) {
+      const int64_t t = t0 + threadIdx.x * 8;
+      uint64_t w;
+      __builtin_memcpy(&w, m + t, 8);
+      if (w) {
+        see(t + (__ffsll(static_cast<unsigned long long>(w)) - 1) / 8, true);
+        see(t + (63 - __clzll(static_cast<long long>(w))) / 8, true);
+      }
     }
   }
+  for (int64_t t = t0 + threadIdx.x; t < seen; t += 256) see(t, kept(t));
   atomicMin(&lo_s, lo);
   atomicMax(&hi_s, hi);
   __syncthreads();
@@ -423,13 +482,13 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   } else {
     launch_vector<TQ_DTYPE_BF16>(p, k_bits, v_bits, n_blocks, st);
   }
-  const unsigned out_rows = static_cast<unsigned>(rows_of(B, Hq, L));
+  const int64_t out_rows = rows_of(B, Hq, L);
   if (q_dtype == TQ_DTYPE_F32)
-    affine_merge_kernel<TQ_DTYPE_F32><<<out_rows, 256, 0, st>>>(p);
+    launch_merge<TQ_DTYPE_F32>(p, out_rows, st);
   else if (q_dtype == TQ_DTYPE_F16)
-    affine_merge_kernel<TQ_DTYPE_F16><<<out_rows, 256, 0, st>>>(p);
+    launch_merge<TQ_DTYPE_F16>(p, out_rows, st);
   else
-    affine_merge_kernel<TQ_DTYPE_BF16><<<out_rows, 256, 0, st>>>(p);
+    launch_merge<TQ_DTYPE_BF16>(p, out_rows, st);
   return check_launch("tq_attention_affine");
 }
 

@@ -33,9 +33,18 @@ struct TileShape {
   static constexpr int DK = 32 * KS, DV = 16 * CT;
   static constexpr int RT = KS <= 4 && CT <= 8 ? 2 : 1;  // 16-row tiles a wave
   static constexpr int ROWS = kTileWaves * 16 * RT;
-  static constexpr int KROW = DK + 8;          // 16-bit elements of a token's row of keys in LDS
-  static constexpr int VROW = kTileStep + 8;   // of a coordinate's row of values
+  // 16-byte pieces in LDS.  Sixteen lanes read one piece of sixteen rows, four pieces at once; a read is served in groups
+  // of lanes that mix rows and pieces, so a piece's place is its number xor the row's (or half the row's, where two
+  // rows span the banks): any such group then meets every bank once.  Rows of 12 or 24 pieces are padded instead.
+  static constexpr bool SWIZZLE = KS == 2 || KS == 4 || KS == 8;
+  static constexpr int KROW = DK + (SWIZZLE ? 0 : 8);  // 16-bit elements of a token's row of keys
+  static constexpr int VROW = kTileStep;               // of a coordinate's row of values
   static constexpr int KBUF = kTileStep * KROW, VBUF = DV * VROW;
+  __device__ static __forceinline__ int k_at(int tok, int piece) {
+    const int place = !SWIZZLE ? piece : KS == 2 ? piece ^ ((tok >> 1) & 7) : piece ^ (tok & 15);
+    return tok * KROW + place * 8;
+  }
+  __device__ static __forceinline__ int v_at(int d, int piece) { return d * VROW + (piece ^ ((d >> 1) & 7)) * 8; }
   static constexpr int KU = KS;                // 8-coordinate pieces of keys a decoding thread has (256 threads)
   static constexpr int VU = (CT + 7) / 8;      // (4 tokens x 8 coordinates) units of values
 };
@@ -92,7 +101,7 @@ __device__ __forceinline__ float cut(float2 sb, float code) {
   return fminf(fmaxf(__builtin_fmaf(sb.x, code, sb.y), -most), most);
 }
 
-template <int DT, int KB, int VB, int KS, int CT>
+template <int DT, int KB, int VB, int KS, int CT, bool MASK>
 __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const AffineAttnParams p, const MaskRows mrows) {
   using S = TileShape<KS, CT>;
   constexpr int RT = S::RT;
@@ -115,7 +124,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 
   // tokens that any row of this workgroup sees
   int first = static_cast<int>(start), stop = static_cast<int>(end);
-  if (p.mask_kind != TQ_MASK_NONE) {
+  if constexpr (MASK) {
     if (tid == 0) range_lds[0] = stop, range_lds[1] = first;
     __syncthreads();
     int lo = stop, hi = first;
@@ -157,10 +166,10 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
       if (p.scale < 0.f) qop[rt][s] ^= u32x4_t{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
     }
     lim[rt] = p.causal ? static_cast<int>(end) - p.L + l : INT32_MAX;
-    mask_at[rt] = p.mask_kind != TQ_MASK_NONE
-                      ? b * p.mask_s[0] + h * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3] : 0;
+    mask_at[rt] = MASK ? b * p.mask_s[0] + h * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3] : 0;
   }
   const float scale = fabsf(p.scale);
+  const bool quads = MASK && p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1;
   // the causal rule leaves a step of tokens alone when its last one is within the first row's limit
   const int lim_min = p.causal ? static_cast<int>(end) - p.L + row0 / p.R : INT32_MAX;
 
@@ -183,14 +192,24 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
   constexpr int KREGS = S::KU * (KWORDS + 1), VREGS = S::VU * 4 * (VWORDS + 1);
   uint32_t raw[KREGS > VREGS ? KREGS : VREGS];
 
+  // The thread's number within its half, by a way that the compiler does not look through: it would keep every address
+  // made from it for the whole loop, past what the registers hold, and fetching one back from scratch memory waits for
+  // all codes on their way.
+  auto half_id = [&]() {
+    uint32_t id = dtid;
+    asm volatile("" : "+v"(id));
+    return id;
+  };
+
   auto load = [&](int t) {
     const int last = min(t1 - t, kTileStep) - 1;
+    const uint32_t id = half_id();
     if (keys) {
       const uint32_t* codes = p.k_codes + (base + t) * (S::DK * KB / 32);
       const uint32_t* pairs = static_cast<const uint32_t*>(p.k_params) + (base + t) * (S::DK >> (shift + 3));
 #pragma unroll
       for (int i = 0; i < S::KU; ++i) {
-        const uint32_t unit = i * 256 + dtid;
+        const uint32_t unit = i * 256 + id;
         const uint32_t tok = min(static_cast<int>(unit / (KS * 4)), last), piece = unit % (KS * 4);
         const uint32_t at = (tok * (S::DK * KB / 32) + piece * KWORDS) * 4;
         if constexpr (KWORDS == 1) {
@@ -206,7 +225,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
       const uint32_t* pairs = static_cast<const uint32_t*>(p.v_params) + (base + t) * (S::DV >> (shift + 3));
 #pragma unroll
       for (int i = 0; i < S::VU; ++i) {
-        const uint32_t unit = i * 256 + dtid;
+        const uint32_t unit = i * 256 + id;
         const uint32_t quad = unit % 16, piece = min(unit / 16, static_cast<uint32_t>(CT * 2 - 1));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -225,11 +244,12 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
     }
   };
 
-  auto decode = [&](int buf, int flags) {
-    if (keys) {
+  auto decode_keys = [&](int buf) {
+    const uint32_t id = half_id();
+    {
 #pragma unroll
       for (int i = 0; i < S::KU; ++i) {
-        const uint32_t unit = i * 256 + dtid;
+        const uint32_t unit = i * 256 + id;
         const uint32_t tok = unit / (KS * 4), piece = unit % (KS * 4);
         const uint32_t* w = raw + i * (KWORDS + 1);
         const float2 sb = pair16<DT>(w[KWORDS]);
@@ -247,12 +267,16 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
             o[j] = nan ? pack_of<DT>(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y))
                        : pack_of<DT>(cut<DT>(sb, f[2 * j]), cut<DT>(sb, f[2 * j + 1]));
         }
-        *reinterpret_cast<u32x4_t*>(&k_lds[buf][tok * S::KROW + piece * 8]) = o;
+        *reinterpret_cast<u32x4_t*>(&k_lds[buf][S::k_at(tok, piece)]) = o;
       }
-    } else {
+    }
+  };
+  auto decode_values = [&](int buf, int flags) {
+    const uint32_t id = half_id();
+    {
 #pragma unroll
       for (int i = 0; i < S::VU; ++i) {
-        const uint32_t unit = i * 256 + dtid;
+        const uint32_t unit = i * 256 + id;
         const uint32_t quad = unit % 16, piece = unit / 16;
         if (piece >= CT * 2) break;
         float v[4][8];
@@ -276,7 +300,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint2 two = make_uint2(pack_of<DT>(v[0][e], v[1][e]), pack_of<DT>(v[2][e], v[3][e]));
-          *reinterpret_cast<uint2*>(&v_lds[buf][(piece * 8 + e) * S::VROW + pos]) = two;
+          *reinterpret_cast<uint2*>(&v_lds[buf][S::v_at(piece * 8 + e, pos >> 3) + (pos & 4)]) = two;
         }
       }
     }
@@ -286,7 +310,10 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
   __syncthreads();
   if (t0 < t1) {
     load(t0);
-    decode(0, 0);
+    if (keys)
+      decode_keys(0);
+    else
+      decode_values(0, 0);
     if (t0 + kTileStep < t1) load(t0 + kTileStep);
   }
   __syncthreads();
@@ -294,28 +321,65 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
   int buf = 0, flags = 0;  // flags: a step's, the next's (written now) and the one after (cleared now)
   for (int t = t0; t < t1; t += kTileStep, buf ^= 1, flags = flags == 2 ? 0 : flags + 1) {
     const bool more = t + kTileStep < t1;
+    // four tokens' bytes of a contiguous boolean mask, on their way while the scores are computed
+    uint32_t quad[RT][4];
+    const bool by_quads = quads && t + kTileStep <= t1;
+    if (MASK && by_quads) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti)
+          __builtin_memcpy(&quad[rt][ti], static_cast<const uint8_t*>(p.mask) + mask_at[rt] + t + ti * 16 + q4 * 4, 4);
+    }
+    // The next tile goes into the other half of LDS, and its successor's codes on their way: the waves of the values do
+    // it here, the waves of the keys at the end, so that of a SIMD's two waves one is at vector work while the other is
+    // at matrix work all through the step.
+    if (tid < 2) bad_lds[flags == 0 ? 2 : flags - 1][tid] = 0;
+    if (!keys && more) decode_values(buf ^ 1, flags == 2 ? 0 : flags + 1);
+    if (!MASK && !keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
     // ---- scores
+    // operands a tile ahead of the products: a read of LDS takes longer than the products of the one before
     f32x4_t C[RT][4];
+    u32x4_t kop[2][KS];
+    auto read_keys = [&](int ti) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        kop[ti & 1][s] = *reinterpret_cast<const u32x4_t*>(&k_lds[buf][S::k_at(ti * 16 + c, s * 4 + q4)]);
+    };
+    read_keys(0);
 #pragma unroll
     for (int ti = 0; ti < 4; ++ti) {
+      if (ti < 3) read_keys(ti + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) C[rt][ti] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const u32x4_t k = *reinterpret_cast<const u32x4_t*>(&k_lds[buf][(ti * 16 + c) * S::KROW + s * 32 + q4 * 8]);
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) C[rt][ti] = mfma_of<DT>(k, qop[rt][s], C[rt][ti]);
-      }
+        for (int rt = 0; rt < RT; ++rt) C[rt][ti] = mfma_of<DT>(kop[ti & 1][s], qop[rt][s], C[rt][ti]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // the next tile into the other half of LDS, and its successor's codes on their way
-    if (tid < 2) bad_lds[flags == 0 ? 2 : flags - 1][tid] = 0;
-    if (more) {
-      decode(buf ^ 1, flags == 2 ? 0 : flags + 1);
-      if (t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
+    if (MASK && by_quads) {  // the mask has arrived here, so that nothing later waits for it and the codes behind it
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti) asm volatile("" : "+v"(quad[rt][ti]));
     }
+    if (MASK && !keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
 
     // ---- softmax
-    const bool plain = p.mask_kind == TQ_MASK_NONE && t + kTileStep - 1 <= lim_min && t + kTileStep <= t1;
+    bool plain = !MASK && t + kTileStep - 1 <= lim_min && t + kTileStep <= t1;
+    if (MASK && by_quads && t + kTileStep - 1 <= lim_min) {  // every byte of the tile set: nothing to mask
+      bool hidden = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int ti = 0; ti < 4; ++ti) {
+          const uint32_t w = quad[rt][ti];
+          hidden |= ((w - 0x01010101u) & ~w & 0x80808080u) != 0;  // a byte of w is 0
+        }
+      plain = !__any(hidden);
+    }
     u32x4_t A[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -335,7 +399,10 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
           for (int j = 0; j < 4; ++j) {
             float y = C[rt][ti][j] * scale;
             const int tok = t + ti * 16 + q4 * 4 + j;
-            if (p.mask_kind != TQ_MASK_NONE) y = affine_mask(p, mask_at[rt] + min(tok, t1 - 1) * p.mask_s[4], y);
+            if (MASK && by_quads)
+              y = (quad[rt][ti] >> (8 * j)) & 0xffu ? y : -FLT_MAX;
+            else if constexpr (MASK)
+              y = affine_mask(p, mask_at[rt] + min(tok, t1 - 1) * p.mask_s[4], y);
             if (tok > lim[rt] && y != -INFINITY) y = -FLT_MAX;
             if (tok >= t1) y = -INFINITY;
             C[rt][ti][j] = y;
@@ -381,19 +448,33 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
         }
     }
 
-    // ---- values
+    // ---- values: groups of VG operands, one ahead of the products
     constexpr uint32_t kOnes = DT == TQ_DTYPE_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    constexpr int VG = KS == 8 ? 2 : CT % 4 == 0 ? 4 : 3, NGR = CT / VG;
     const u32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
+    u32x4_t vop[2][VG];
+    auto read_values = [&](int at) {  // group at % NGR of the half step at / NGR
 #pragma unroll
-    for (int pr = 0; pr < 2; ++pr) {
+      for (int i = 0; i < VG; ++i)
+        vop[at & 1][i] = *reinterpret_cast<const u32x4_t*>(
+            &v_lds[buf][S::v_at(((at % NGR) * VG + i) * 16 + c, (at / NGR) * 4 + q4)]);
+    };
+    read_values(0);
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma_of<DT>(A[rt][pr], ones, sum[rt]);
+    for (int at = 0; at < 2 * NGR; ++at) {
+      const int pr = at / NGR;
+      if (at + 1 < 2 * NGR) read_values(at + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (at % NGR == 0) {
 #pragma unroll
-      for (int n = 0; n < CT; ++n) {
-        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(&v_lds[buf][(n * 16 + c) * S::VROW + pr * 32 + q4 * 8]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][n] = mfma_of<DT>(A[rt][pr], v, acc[rt][n]);
+        for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma_of<DT>(A[rt][pr], ones, sum[rt]);
       }
+#pragma unroll
+      for (int i = 0; i < VG; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][(at % NGR) * VG + i] = mfma_of<DT>(A[rt][pr], vop[at & 1][i], acc[rt][(at % NGR) * VG + i]);
+      __builtin_amdgcn_sched_barrier(0);
     }
 
     // ---- tokens whose values are not finite, for the rows that weigh them
@@ -405,11 +486,14 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
         const int64_t at = base + t + tok;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          float w = 0.f;
+          // the rounded weight: tile tok / 16, two tokens a register
+          uint32_t two = 0;
 #pragma unroll
-          for (int ti = 0; ti < 4; ++ti)
+          for (int pr = 0; pr < 2; ++pr)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w = tok / 16 == ti && tok % 4 == j ? C[rt][ti][j] : w;
+            for (int j = 0; j < 4; ++j) two = tok / 32 == pr && tok / 16 % 2 * 2 + tok % 4 / 2 == j ? A[rt][pr][j] : two;
+          const float2 both = pair16<DT>(two);
+          const float w = tok % 2 ? both.y : both.x;
           float wr[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) wr[j] = __shfl(w, (tok % 16) / 4 * 16 + q4 * 4 + j);
@@ -426,6 +510,8 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
         }
       }
     }
+    if (keys && more) decode_keys(buf ^ 1);
+    if (keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
     __syncthreads();
   }
 
@@ -459,7 +545,10 @@ int launch_tile_at(const AffineAttnParams& p, const MaskRows& m, hipStream_t st)
   static_assert(kRows == tile_rows(32 * KS, 16 * CT), "rows a workgroup");
   const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * ((p.rows + kRows - 1) / kRows) * p.splits;
   if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
-  affine_tile_kernel<DT, KB, VB, KS, CT><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
+  if (p.mask_kind != TQ_MASK_NONE)
+    affine_tile_kernel<DT, KB, VB, KS, CT, true><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
+  else
+    affine_tile_kernel<DT, KB, VB, KS, CT, false><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
   return check_launch("affine_tile_kernel");
 }
 
