@@ -10,10 +10,15 @@ An ``AffineState`` holds the codes and the (scale, bias) pairs; its head dim
 and bit width follow from its shapes and the group size.  Functions check
 their arguments on the host, run on torch's current stream of the tensors'
 device and raise as the other wrappers of this package do.
+
+What follows from shapes, strides and types alone (the checks, the layout, the
+workspace's size) is worked out once for each such set and remembered: a short
+decode step waits for the host (one call 20 -> 11 us of it).
 """
 from __future__ import annotations
 
 import contextlib
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -73,59 +78,96 @@ def affine_state(B: int, H: int, capacity: int, dim: int, bits: int, group_size:
 
 
 def _same_device(*ts: torch.Tensor) -> None:
-    ops._require_device(*ts)
-    if any(t.device != ts[0].device for t in ts[1:]):
+    """Raises unless all tensors are on one ROCm device."""
+    try:
+        d = ts[0].get_device()
+        same = d >= 0
+        for t in ts:
+            same &= t.get_device() == d
+    except AttributeError:  # not a tensor
+        same = False
+    if not same:
+        ops._require_device(*ts)
         raise ValueError(f"tensors are on different devices: {[str(t.device) for t in ts]}")
 
 
-def _shape_of(st: AffineState, group_size: int, what: str) -> Tuple[int, int]:
-    """(dim, bits) of a state from its shapes."""
-    c, p = st.codes, st.params
-    if c.dim() != 4 or p.dim() != 5 or p.shape[4] != 2 or c.shape[:3] != p.shape[:3]:
-        raise ValueError(f"{what} state of shapes {tuple(c.shape)} / {tuple(p.shape)} is not "
+@functools.lru_cache(maxsize=1024)
+def _layout(c_shape, c_stride, c_dtype, p_shape, p_stride, group_size: int, what: str) -> Tuple[int, int, int]:
+    """(dim, bits, capacity) of a state that views a token range of contiguous
+    (B, H, cap, ...) buffers, from its shapes and strides."""
+    _check_group(group_size)
+    if len(c_shape) != 4 or len(p_shape) != 5 or p_shape[4] != 2 or c_shape[:3] != p_shape[:3]:
+        raise ValueError(f"{what} state of shapes {tuple(c_shape)} / {tuple(p_shape)} is not "
                          "(B, H, T, words) codes and (B, H, T, groups, 2) params")
-    if c.dtype != torch.uint32:
-        raise ValueError(f"{what} codes must be uint32, got {c.dtype}")
-    dim = _check_dim(p.shape[3] * group_size, group_size, what)
-    for bits in BITS:
-        if c.shape[3] * 32 == dim * bits:
-            return dim, bits
-    raise ValueError(f"{what} rows of {c.shape[3]} words hold no {dim} codes of 4 or 8 bits")
+    if c_dtype != torch.uint32:
+        raise ValueError(f"{what} codes must be uint32, got {c_dtype}")
+    B, H, T, pw = c_shape
+    dim = _check_dim(p_shape[3] * group_size, group_size, what)
+    bits = next((b for b in BITS if pw * 32 == dim * b), None)
+    if bits is None:
+        raise ValueError(f"{what} rows of {pw} words hold no {dim} codes of 4 or 8 bits")
+    pg = 2 * p_shape[3]
+    cap = c_stride[1] // pw if H > 1 else c_stride[0] // pw if B > 1 else max(T, 1)
+    if B * H * T > 0:
+        ok = c_stride[3] == 1 and p_stride[4] == 1 and (p_shape[3] == 1 or p_stride[3] == 2) and cap >= T
+        ok = ok and (T <= 1 or (c_stride[2] == pw and p_stride[2] == pg))
+        if H > 1:
+            ok = ok and c_stride[1] == cap * pw and p_stride[1] == cap * pg
+        if B > 1:
+            ok = ok and c_stride[0] == H * cap * pw and p_stride[0] == H * cap * pg
+        if not ok:
+            raise ValueError(f"{what} state must view one token range of contiguous (B, H, cap, {pw}) codes and "
+                             f"(B, H, cap, {p_shape[3]}, 2) params")
+    return dim, bits, cap
 
 
 def _check_aligned(st: AffineState, what: str) -> None:
     """Rows of codes are whole 16-byte pieces; a (scale, bias) pair is loaded at once."""
-    if st.codes.data_ptr() & 15 or st.params.data_ptr() % (2 * st.params.element_size()):
+    codes, params = st
+    if codes.data_ptr() & 15 or params.data_ptr() % (2 * params.element_size()):
         raise ValueError(f"{what} state is not aligned (16 bytes of codes, a pair of params)")
 
 
-def _capacity(st: AffineState, what: str) -> int:
-    """Token capacity of the contiguous (B, H, cap, ...) buffers that a state views a token range of."""
-    c, p = st.codes, st.params
-    B, H, T, pw = c.shape
-    pg = 2 * p.shape[3]
-    cap = c.stride(1) // pw if H > 1 else c.stride(0) // pw if B > 1 else max(T, 1)
-    ok = c.stride(3) == 1 and p.stride(4) == 1 and (p.shape[3] == 1 or p.stride(3) == 2) and cap >= T
-    ok = ok and (T <= 1 or (c.stride(2) == pw and p.stride(2) == pg))
-    if H > 1:
-        ok = ok and c.stride(1) == cap * pw and p.stride(1) == cap * pg
-    if B > 1:
-        ok = ok and c.stride(0) == H * cap * pw and p.stride(0) == H * cap * pg
-    if not ok:
-        raise ValueError(f"{what} state must view one token range of contiguous (B, H, cap, {pw}) codes and "
-                         f"(B, H, cap, {p.shape[3]}, 2) params")
-    _check_aligned(st, what)
-    return cap
+def _is_contiguous(shape, stride) -> bool:
+    want = 1
+    for n, st in zip(reversed(shape), reversed(stride)):
+        if n != 1 and st != want:
+            return False
+        want *= max(n, 1)
+    return True
 
 
 def _vectors(x: torch.Tensor) -> torch.Tensor:
     """x with a contiguous, 16-byte aligned last axis (compacted where it has none)."""
-    if x.stride(-1) != 1:
-        return x.contiguous()
-    sb, sh, sl, _ = x.stride()
-    if (x.data_ptr() | (sb | sh | sl) * x.element_size()) & 15:
-        return x.contiguous()
+    sb, sh, sl, sd = x.stride()
+    if sd != 1 or (x.data_ptr() | (sb | sh | sl) * x.element_size()) & 15:
+        return x.clone(memory_format=torch.contiguous_format)  # a contiguous x may start off 16 bytes too
     return x
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_plan(k_shape, v_shape, k_dtype, v_dtype, kc_shape, kc_stride, kc_dtype, kp_shape, kp_stride, kp_dtype,
+                 vc_shape, vc_stride, vc_dtype, vp_shape, vp_stride, vp_dtype, group_size):
+    """(key bits, value bits, capacity) of an append whose shapes and types fit."""
+    _check_group(group_size)
+    if len(k_shape) != 4 or len(v_shape) != 4 or v_shape[:3] != k_shape[:3]:
+        raise ValueError(f"keys {tuple(k_shape)} and values {tuple(v_shape)} must share (B, H, L)")
+    bits = []
+    for shape, dtype, cs, ct, cd, ps, pt, pd, what in (
+            (k_shape, k_dtype, kc_shape, kc_stride, kc_dtype, kp_shape, kp_stride, kp_dtype, "key"),
+            (v_shape, v_dtype, vc_shape, vc_stride, vc_dtype, vp_shape, vp_stride, vp_dtype, "value")):
+        dim, b, _ = _layout(cs, ct, cd, ps, pt, group_size, what)
+        if shape[3] != dim:
+            raise ValueError(f"{what} head dim {shape[3]} != the state's {dim}")
+        if dtype != pd or dtype != k_dtype:
+            raise ValueError(f"{what}s of {dtype} for a state of {pd} and keys of {k_dtype}")
+        if not (_is_contiguous(cs, ct) and _is_contiguous(ps, pt)):
+            raise ValueError("cache buffers must be contiguous")
+        if cs[:2] != k_shape[:2] or cs[2] != kc_shape[2]:
+            raise ValueError(f"{what} buffers {tuple(cs)} do not match ({k_shape[0]}, {k_shape[1]}, capacity)")
+        bits.append(b)
+    _lib.torch_dtype_code(k_dtype)
+    return bits[0], bits[1], kc_shape[2]
 
 
 def append_affine_kv(k: torch.Tensor, v: torch.Tensor, k_state: AffineState, v_state: AffineState, offset: int,
@@ -140,34 +182,22 @@ def append_affine_kv(k: torch.Tensor, v: torch.Tensor, k_state: AffineState, v_s
     """
     if not _direct and torch.compiler.is_compiling():
         return torch.ops.kaplumba.append_affine_kv(k, v, *k_state, *v_state, offset, group_size)
-    _same_device(k, v, *k_state, *v_state)
-    _check_group(group_size)
-    if k.dim() != 4 or v.shape[:3] != k.shape[:3] or v.dim() != 4:
-        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} must share (B, H, L)")
+    kc, kp = k_state
+    vc, vp = v_state
+    _same_device(k, v, kc, kp, vc, vp)
+    kb, vb, cap = _append_plan(k.shape, v.shape, k.dtype, v.dtype, kc.shape, kc.stride(), kc.dtype, kp.shape, kp.stride(),
+                               kp.dtype, vc.shape, vc.stride(), vc.dtype, vp.shape, vp.stride(), vp.dtype, group_size)
+    _check_aligned(k_state, "key")
+    _check_aligned(v_state, "value")
     B, H, L, Dk = k.shape
-    sides = []
-    for x, st, what in ((k, k_state, "key"), (v, v_state, "value")):
-        dim, bits = _shape_of(st, group_size, what)
-        if x.shape[-1] != dim:
-            raise ValueError(f"{what} head dim {x.shape[-1]} != the state's {dim}")
-        if x.dtype != st.params.dtype or x.dtype != k.dtype:
-            raise ValueError(f"{what}s of {x.dtype} for a state of {st.params.dtype} and keys of {k.dtype}")
-        if not (st.codes.is_contiguous() and st.params.is_contiguous()):
-            raise ValueError("cache buffers must be contiguous")
-        if st.codes.shape[:2] != (B, H) or st.codes.shape[2] != k_state.codes.shape[2]:
-            raise ValueError(f"{what} buffers {tuple(st.codes.shape)} do not match ({B}, {H}, capacity)")
-        _check_aligned(st, what)
-        sides.append(bits)
-    cap = k_state.codes.shape[2]
     if not 0 <= offset <= cap - L:
         raise ValueError(f"rows {offset}..{offset + L} are outside the capacity of {cap}")
     k, v = _vectors(k), _vectors(v)
     with _device_guard(k):
         rc = _lib.load().tq_append_affine_kv(
             k.data_ptr(), v.data_ptr(), _lib.torch_dtype_code(k.dtype), B, H, L, Dk, v.shape[-1],
-            k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), sides[0], sides[1],
-            group_size, k_state.codes.data_ptr(), k_state.params.data_ptr(), v_state.codes.data_ptr(),
-            v_state.params.data_ptr(), cap, offset, ops._stream(k))
+            *k.stride()[:3], *v.stride()[:3], kb, vb, group_size, kc.data_ptr(), kp.data_ptr(), vc.data_ptr(),
+            vp.data_ptr(), cap, offset, ops._stream(k))
     _lib.check(rc, "tq_append_affine_kv")
 
 
@@ -175,23 +205,51 @@ def dequantize_affine(state: AffineState, group_size: int = 64, dtype: Optional[
                       _direct: bool = False) -> torch.Tensor:
     """(B, H, T, dim) values ``scale * code + bias`` of a state (a token range of its
     buffers), computed in f32 and rounded once to ``dtype`` (default: the state's)."""
-    dtype = dtype or state.params.dtype
+    c, p = state
+    dtype = dtype or p.dtype
     if not _direct and torch.compiler.is_compiling():
-        return torch.ops.kaplumba.dequantize_affine(*state, group_size, dtype)
-    _same_device(*state)
-    dim, bits = _shape_of(state, _check_group(group_size), "cache")
-    B, H, T = state.codes.shape[:3]
-    out = torch.empty((B, H, T, dim), dtype=dtype, device=state.codes.device)
-    code_in, code_out = _lib.torch_dtype_code(state.params.dtype), _lib.torch_dtype_code(dtype)
-    if out.numel() == 0:
+        return torch.ops.kaplumba.dequantize_affine(c, p, group_size, dtype)
+    _same_device(c, p)
+    dim, bits, cap = _layout(c.shape, c.stride(), c.dtype, p.shape, p.stride(), group_size, "cache")
+    B, H, T, _ = c.shape
+    out = torch.empty((B, H, T, dim), dtype=dtype, device=c.device)
+    code_in, code_out = _lib.torch_dtype_code(p.dtype), _lib.torch_dtype_code(dtype)
+    if B * H * T == 0:
         return out
-    cap = _capacity(state, "cache")
+    _check_aligned(state, "cache")
     with _device_guard(out):
-        rc = _lib.load().tq_dequantize_affine(
-            state.codes.data_ptr(), state.params.data_ptr(), code_in, B, H, T, dim, bits, group_size, cap,
-            out.data_ptr(), code_out, ops._stream(out))
+        rc = _lib.load().tq_dequantize_affine(c.data_ptr(), p.data_ptr(), code_in, B, H, T, dim, bits, group_size, cap,
+                                              out.data_ptr(), code_out, ops._stream(out))
     _lib.check(rc, "tq_dequantize_affine")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_plan(q_shape, q_dtype, kc_shape, kc_stride, kc_dtype, kp_shape, kp_stride, kp_dtype, vc_shape, vc_stride,
+                    vc_dtype, vp_shape, vp_stride, vp_dtype, group_size):
+    """What an attention call's shapes and types come to, once they fit:
+    (Hkv, T, Dv, key bits, value bits, capacity, dtype code, workspace bytes)."""
+    _check_group(group_size)
+    if len(q_shape) != 4:
+        raise ValueError(f"queries must be (B, Hq, L, D), got {tuple(q_shape)}")
+    B, Hq, L, Dk = q_shape
+    dim, kb, cap = _layout(kc_shape, kc_stride, kc_dtype, kp_shape, kp_stride, group_size, "key")
+    Dv, vb, vcap = _layout(vc_shape, vc_stride, vc_dtype, vp_shape, vp_stride, group_size, "value")
+    Hkv, T = kc_shape[1], kc_shape[2]
+    if dim != Dk:
+        raise ValueError(f"query head dim {Dk} != key head dim {dim}")
+    if kc_shape[0] != B or vc_shape[:3] != kc_shape[:3]:
+        raise ValueError(f"queries of batch {B}, keys {tuple(kc_shape[:3])} and values {tuple(vc_shape[:3])} must share "
+                         "(B, Hkv, T)")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are not a multiple of {Hkv} kv heads")
+    if not q_dtype == kp_dtype == vp_dtype:
+        raise ValueError(f"queries of {q_dtype} over states of {kp_dtype} and {vp_dtype}")
+    code = _lib.torch_dtype_code(q_dtype)
+    if B * Hq * L * T and vcap != cap:
+        raise ValueError("key and value buffers must share a capacity")
+    ws = _lib.load().tq_attention_affine_workspace_size(B, Hq, Hkv, L, Dk, Dv, T)
+    return Hkv, T, Dv, kb, vb, cap, code, ws
 
 
 def attention_affine(queries: torch.Tensor, k_state: AffineState, v_state: AffineState, group_size: int = 64,
@@ -211,47 +269,34 @@ def attention_affine(queries: torch.Tensor, k_state: AffineState, v_state: Affin
             queries, *k_state, *v_state, group_size, float(scale), bool(causal),
             ops._opt_tensor(seq_lens, torch.int32), ops._opt_tensor(seq_starts, torch.int32),
             ops._opt_tensor(mask, None))
-    _same_device(queries, *k_state, *v_state)
-    if torch.is_grad_enabled() and queries.requires_grad:
+    kc, kp = k_state
+    vc, vp = v_state
+    _same_device(queries, kc, kp, vc, vp)
+    if queries.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("attention_affine has no backward pass: call it under torch.no_grad()")
-    _check_group(group_size)
-    if queries.dim() != 4:
-        raise ValueError(f"queries must be (B, Hq, L, D), got {tuple(queries.shape)}")
+    Hkv, T, Dv, kb, vb, cap, dtype, ws_bytes = _attention_plan(
+        queries.shape, queries.dtype, kc.shape, kc.stride(), kc.dtype, kp.shape, kp.stride(), kp.dtype, vc.shape,
+        vc.stride(), vc.dtype, vp.shape, vp.stride(), vp.dtype, group_size)
     B, Hq, L, Dk = queries.shape
-    dim, kb = _shape_of(k_state, group_size, "key")
-    Dv, vb = _shape_of(v_state, group_size, "value")
-    Hkv, T = k_state.codes.shape[1], k_state.codes.shape[2]
-    if dim != Dk:
-        raise ValueError(f"query head dim {Dk} != key head dim {dim}")
-    if k_state.codes.shape[0] != B or v_state.codes.shape[:3] != k_state.codes.shape[:3]:
-        raise ValueError(f"queries of batch {B}, keys {tuple(k_state.codes.shape[:3])} and values "
-                         f"{tuple(v_state.codes.shape[:3])} must share (B, Hkv, T)")
-    if Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"{Hq} query heads are not a multiple of {Hkv} kv heads")
-    if not queries.dtype == k_state.params.dtype == v_state.params.dtype:
-        raise ValueError(f"queries of {queries.dtype} over states of {k_state.params.dtype} and {v_state.params.dtype}")
-    dtype = _lib.torch_dtype_code(queries.dtype)
-    out = torch.empty((B, Hq, L, Dv), dtype=queries.dtype, device=queries.device)
-    if out.numel() == 0:
-        return out
-    if T == 0:
+    if Dv == Dk:
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+    else:
+        out = queries.new_empty((B, Hq, L, Dv))
+    if B * Hq * L * T == 0:
         return out.zero_()
-    cap = _capacity(k_state, "key")
-    if _capacity(v_state, "value") != cap:
-        raise ValueError("key and value buffers must share a capacity")
+    _check_aligned(k_state, "key")
+    _check_aligned(v_state, "value")
     queries = _vectors(queries)
     seq_lens = ops._seq_array(seq_lens, B, queries.device)
     seq_starts = ops._seq_array(seq_starts, B, queries.device)
     mt, mkind, mstr = None, _lib.TQ_MASK_NONE, None
     if mask is not None:
         mt, mkind, mstr = ops.prepare_mask(mask, B, Hkv, Hq // Hkv, L, T, queries.device, grouped=False)
-    lib = _lib.load()
     with _device_guard(queries):
-        ws = ops._workspace(queries.device, lib.tq_attention_affine_workspace_size(B, Hq, Hkv, L, Dk, Dv, T))
-        rc = lib.tq_attention_affine(
-            queries.data_ptr(), dtype, B, Hq, Hkv, L, Dk, Dv, queries.stride(0), queries.stride(1),
-            queries.stride(2), float(scale), k_state.codes.data_ptr(), k_state.params.data_ptr(), kb,
-            v_state.codes.data_ptr(), v_state.params.data_ptr(), vb, group_size, cap, T,
+        ws = ops._workspace(queries.device, ws_bytes)
+        rc = _lib.load().tq_attention_affine(
+            queries.data_ptr(), dtype, B, Hq, Hkv, L, Dk, Dv, *queries.stride()[:3], float(scale), kc.data_ptr(),
+            kp.data_ptr(), kb, vc.data_ptr(), vp.data_ptr(), vb, group_size, cap, T,
             seq_starts.data_ptr() if seq_starts is not None else None,
             seq_lens.data_ptr() if seq_lens is not None else None, 1 if causal else 0,
             mt.data_ptr() if mt is not None else None, mkind, mstr, out.data_ptr(), ws.data_ptr(), ws.numel(),

@@ -7,6 +7,7 @@ with query and key norms take those first.  Positions may have several axes
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -19,35 +20,47 @@ __all__ = ["norm_rope"]
 PAIRS = ("half", "adjacent")
 
 
-def _positions(positions, axis, B: int, L: int, device):
-    """(tensor or None, start, strides over (axis, b, l), number of axes)."""
-    if not isinstance(positions, torch.Tensor):
-        if axis is not None:
+@functools.lru_cache(maxsize=1024)
+def _plan(q_shape, q_dtype, k_shape, k_dtype, pos_shape, pos_stride, pos_dtype, inv_shape, axis_shape, axis_dtype,
+          qw_shape, kw_shape, pairs):
+    """What a call's shapes and types come to, once they fit: (Hk, dtype code, rotated coordinates, axes, position
+    bytes, position strides over (axis, b, l))."""
+    if len(q_shape) != 4 or len(k_shape) != 4 or q_dtype != k_dtype:
+        raise ValueError(f"queries {tuple(q_shape)} {q_dtype} and keys {tuple(k_shape)} {k_dtype} must be "
+                         "(B, H, L, D) of one dtype")
+    B, Hq, L, D = q_shape
+    Hk = k_shape[1]
+    if k_shape != (B, Hk, L, D):
+        raise ValueError(f"keys {tuple(k_shape)} do not match queries {tuple(q_shape)}")
+    if pairs not in PAIRS:
+        raise ValueError(f"pairs must be one of {PAIRS}, got {pairs!r}")
+    rot = 0
+    if inv_shape is not None:
+        if len(inv_shape) != 1 or 2 * inv_shape[0] > D:
+            raise ValueError(f"inv_freq of shape {tuple(inv_shape)} for a head dim of {D}")
+        rot = 2 * inv_shape[0]
+    if axis_shape is not None and (axis_shape != (rot // 2,) or axis_dtype != torch.int32):
+        raise ValueError(f"axis must be int32 ({rot // 2},), got {axis_dtype} {tuple(axis_shape)}")
+    for shape, what in ((qw_shape, "q"), (kw_shape, "k")):
+        if shape is not None and shape != (D,):
+            raise ValueError(f"{what}_weight of shape {tuple(shape)}: ({D},) is needed")
+    code = _lib.torch_dtype_code(q_dtype)
+    if pos_shape is None:
+        if axis_shape is not None:
             raise ValueError("several axes need a positions tensor (axes, L) or (axes, B, L)")
-        return None, int(positions), (0, 0, 0), 1
-    p = positions
-    if p.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"positions must be int32 or int64, got {p.dtype}")
-    if p.device != device:
-        raise ValueError(f"positions are on {p.device}, the vectors on {device}")
-    lead = 0 if axis is None else 1
-    if p.dim() not in (1 + lead, 2 + lead):
-        raise ValueError(f"positions of shape {tuple(p.shape)} are not " +
+        return Hk, code, rot, 1, 0, (0, 0, 0)
+    if pos_dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {pos_dtype}")
+    lead = 0 if axis_shape is None else 1
+    if len(pos_shape) not in (1 + lead, 2 + lead):
+        raise ValueError(f"positions of shape {tuple(pos_shape)} are not " +
                          ("(axes, L) or (axes, B, L)" if lead else "(L,) or (B, L)"))
-    axes = p.shape[0] if lead else 1
-    if axes < 1 or p.shape[-1] != L or (p.dim() == 2 + lead and p.shape[lead] not in (1, B)):
-        raise ValueError(f"positions of shape {tuple(p.shape)} for {B} sequences of {L} tokens")
-    sa = p.stride(0) if lead else 0
-    sb = p.stride(lead) if p.dim() == 2 + lead and p.shape[lead] == B else 0
-    return p, 0, (sa, sb, p.stride(-1)), axes
-
-
-def _weight(w, dim: int, device, what: str):
-    if w is None:
-        return None
-    if w.shape != (dim,) or w.device != device:
-        raise ValueError(f"{what}_weight of shape {tuple(w.shape)} on {w.device}: ({dim},) on {device} is needed")
-    return w.contiguous()
+    rows = len(pos_shape) == 2 + lead
+    axes = pos_shape[0] if lead else 1
+    if axes < 1 or pos_shape[-1] != L or (rows and pos_shape[lead] not in (1, B)):
+        raise ValueError(f"positions of shape {tuple(pos_shape)} for {B} sequences of {L} tokens")
+    sb = pos_stride[lead] if rows and pos_shape[lead] == B else 0
+    return Hk, code, rot, axes, 4 if pos_dtype == torch.int32 else 8, (pos_stride[0] if lead else 0, sb, pos_stride[-1])
 
 
 def norm_rope(queries: torch.Tensor, keys: torch.Tensor, positions: Union[int, torch.Tensor],
@@ -74,53 +87,47 @@ def norm_rope(queries: torch.Tensor, keys: torch.Tensor, positions: Union[int, t
         return torch.ops.kaplumba.norm_rope(queries, keys, positions if tensor else None,
                                             0 if tensor else positions, inv_freq, axis, q_weight, k_weight,
                                             float(eps), pairs, float(factor))
-    given = [t for t in (inv_freq, axis, q_weight, k_weight) if t is not None]
+    pos = positions if isinstance(positions, torch.Tensor) else None
+    given = [t for t in (inv_freq, axis, q_weight, k_weight, pos) if t is not None]
     _same_device(queries, keys, *given)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (queries, keys, *given)):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in (queries, keys, *given)]):
         raise NotImplementedError("norm_rope has no backward pass: call it under torch.no_grad()")
-    if queries.dim() != 4 or keys.dim() != 4 or queries.dtype != keys.dtype:
-        raise ValueError(f"queries {tuple(queries.shape)} {queries.dtype} and keys {tuple(keys.shape)} {keys.dtype} "
-                         "must be (B, H, L, D) of one dtype")
-    B, Hq, L, D = queries.shape
-    Hk = keys.shape[1]
-    if keys.shape != (B, Hk, L, D):
-        raise ValueError(f"keys {tuple(keys.shape)} do not match queries {tuple(queries.shape)}")
-    if pairs not in PAIRS:
-        raise ValueError(f"pairs must be one of {PAIRS}, got {pairs!r}")
-    rot = 0
-    if inv_freq is not None:
-        if inv_freq.dim() != 1 or 2 * inv_freq.numel() > D:
-            raise ValueError(f"inv_freq of shape {tuple(inv_freq.shape)} for a head dim of {D}")
+    Hk, dtype, rot, axes, pos_bytes, pos_strides = _plan(
+        queries.shape, queries.dtype, keys.shape, keys.dtype, *((pos.shape, pos.stride(), pos.dtype) if pos is not None
+                                                                else (None, None, None)),
+        inv_freq.shape if inv_freq is not None else None, *((axis.shape, axis.dtype) if axis is not None else (None, None)),
+        q_weight.shape if q_weight is not None else None, k_weight.shape if k_weight is not None else None, pairs)
+    start = 0 if pos is not None else int(positions)
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous()):
         inv_freq = inv_freq.to(torch.float32).contiguous()
-        rot = 2 * inv_freq.numel()
     if axis is not None:
-        if axis.shape != (rot // 2,) or axis.dtype != torch.int32:
-            raise ValueError(f"axis must be int32 ({rot // 2},), got {axis.dtype} {tuple(axis.shape)}")
         axis = axis.contiguous()
-    pos, start, (sa, sb, sl), axes = _positions(positions, axis, B, L, queries.device)
-    q_weight = _weight(q_weight, D, queries.device, "q")
-    k_weight = _weight(k_weight, D, queries.device, "k")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        q_weight, k_weight = q_weight.float(), k_weight.float()
-    w = q_weight if q_weight is not None else k_weight
-    dtype = _lib.torch_dtype_code(queries.dtype)
-    wtype = _lib.torch_dtype_code(w.dtype) if w is not None else 0
+    wtype = 0
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+        wtype = q_weight.dtype
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+        if wtype and k_weight.dtype != wtype:
+            q_weight, k_weight = q_weight.float(), k_weight.float()
+        wtype = k_weight.dtype
+    if wtype:
+        wtype = _lib.torch_dtype_code(wtype)
     if queries.stride(-1) != 1:
         queries = queries.contiguous()
     if keys.stride(-1) != 1:
         keys = keys.contiguous()
-    q_out = torch.empty((B, Hq, L, D), dtype=queries.dtype, device=queries.device)
-    k_out = torch.empty((B, Hk, L, D), dtype=keys.dtype, device=keys.device)
-
-    def ptr(t):
-        return t.data_ptr() if t is not None else None
+    B, Hq, L, D = queries.shape
+    q_out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(keys, memory_format=torch.contiguous_format)
 
     with _device_guard(queries):
         rc = _lib.load().tq_norm_rope(
-            queries.data_ptr(), keys.data_ptr(), dtype, B, Hq, Hk, L, D, queries.stride(0), queries.stride(1),
-            queries.stride(2), keys.stride(0), keys.stride(1), keys.stride(2), ptr(q_weight), ptr(k_weight), wtype,
-            float(eps), rot, 1 if pairs == "adjacent" else 0, ptr(inv_freq), float(factor), ptr(axis), axes,
-            ptr(pos), pos.element_size() if pos is not None else 0, start, sa, sb, sl, q_out.data_ptr(),
-            k_out.data_ptr(), ops._stream(queries))
+            queries.data_ptr(), keys.data_ptr(), dtype, B, Hq, Hk, L, D, *queries.stride()[:3], *keys.stride()[:3],
+            q_weight.data_ptr() if q_weight is not None else None,
+            k_weight.data_ptr() if k_weight is not None else None, wtype, float(eps), rot,
+            1 if pairs == "adjacent" else 0, inv_freq.data_ptr() if inv_freq is not None else None, float(factor),
+            axis.data_ptr() if axis is not None else None, axes, pos.data_ptr() if pos is not None else None, pos_bytes,
+            start, *pos_strides, q_out.data_ptr(), k_out.data_ptr(), ops._stream(queries))
     _lib.check(rc, "tq_norm_rope")
     return q_out, k_out

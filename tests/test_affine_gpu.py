@@ -72,7 +72,10 @@ def test_append_strides_and_stream(device):
     x = vectors(3, (B, H, L, 3 * D), torch.bfloat16).to(device)
     k, v = x[..., :D], x[..., D:2 * D].transpose(1, 2).contiguous().transpose(1, 2)
     odd = vectors(4, (B, H, L, D + 1), torch.bfloat16).to(device)[..., 1:]
-    for kk, vv in ((k, v), (odd, v), (k.transpose(2, 3).contiguous().transpose(2, 3), odd)):
+    flat = vectors(5, (1, 1, 1, B * H * L * D + 1), torch.bfloat16).to(device).flatten()
+    off = flat[1:].view(B, H, L, D)                      # contiguous, but not 16-byte aligned
+    assert off.is_contiguous() and off.data_ptr() % 16
+    for kk, vv in ((k, v), (odd, v), (off, v), (k, off), (k.transpose(2, 3).contiguous().transpose(2, 3), odd)):
         ks, vs = (affine_state(B, H, L, D, 4, 64, torch.bfloat16, device) for _ in range(2))
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
