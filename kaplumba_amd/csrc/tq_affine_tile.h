@@ -1,20 +1,26 @@
 // Attention of many query rows (prefill chunks) over the group-affine cache, on the matrix cores.
 //
 // A workgroup takes 8 waves x RT x 16 query rows of one kv head.  Every 64 tokens it decodes keys and values into LDS
-// once for all of them, as the vectors' own type (scale * code + bias in f32, rounded once: an error of half a step a
-// coordinate, as the reference's layers have it, which dequantize in that type), half the waves the keys and half the
-// values, while the tile before is worked on:
-//   scores  C[token][row] = K Q^T (v_mfma_f32_16x16x32), keys row by row in LDS, queries in registers.
+// once for all of them, as f16 (scale * code + bias in f32, rounded once), half the waves the keys and half the values,
+// while the tile before is worked on:
+//   scores  C[token][row] = K Q^T (v_mfma_f32_16x16x32_f16), keys row by row in LDS, queries in registers, each row
+//           times a power of two.
 //   values  O[row][coordinate] = P V: C's lanes hold row = lane % 16 and tokens 4 (lane / 16) + j of every 16-token
 //           tile, which is A's layout when 32 tokens are taken in the order (lane / 16, tile, j); values lie in LDS
 //           transposed and in that order, so weights go from C to A in registers, and the sum of a row's rounded
 //           weights is one more product with ones.
-// Softmax: one reference a row, moved only when a score passes it by 8 (base 2).  Weights go in as one 16-bit number
-// (bf16: 2^-8 of the weight at most; f16: truncated, 2^-10, and up to 2^15 so that small ones stay normal); they are
-// divided by the sum of the same rounded numbers.
+// Softmax: one reference a row, moved only when a score passes it by 8 (base 2).  Weights go in as one f16 (off by 2^-11
+// of themselves, by 2^-25 below 2^-14; of f16 vectors up to 2^15, of bf16 ones up to 2^8, so that large values times
+// weights stay finite); they are divided by the sum of the same rounded numbers.
+// f16 and not the vectors' own type where that is bf16: eight times smaller errors of keys, weights and values.
+// Outputs of 512 bf16 queries over 8192 tokens are then as far from 64 bits as their own rounding (0.0017, against
+// 0.0036 with bf16 operands, 4 us faster); f16 outputs are 0.0005 off where rounding alone is 0.0002.  Exact codes in
+// the products with the pairs in f32 behind them, as few rows have it, take more registers than there are (275 us
+// instead of 109).
 //
-// A token whose values are not finite has zeros in LDS and a flag; the rows that weigh it add it on the vector units,
-// so what a row masks may be NaN.  A group that would leave its type's range when rounded is cut to it.
+// What f16 does not hold (NaN, infinite, past 65504; bf16 groups below 2^-15, where f16's spacing near zero is coarser
+// than bf16's own) is zeros in LDS and a flag for the token: its scores, or its values for the rows that weigh it, are
+// worked out in f32 from the codes, one token at a time.  What a row masks may so be NaN.
 //
 // What bounds it, d = 128, a step of 64 tokens and 256 rows a CU: matrix products 2048 cycles, LDS reads 2048, vector
 // instructions about 2400 a SIMD (softmax 7 a score, decoding 3 an element).
@@ -49,25 +55,18 @@ struct TileShape {
   static constexpr int VU = (CT + 7) / 8;      // (4 tokens x 8 coordinates) units of values
 };
 
-template <int DT>
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
 __device__ __forceinline__ f32x4_t mfma_of(u32x4_t a, u32x4_t b, f32x4_t c) {
-  if constexpr (DT == TQ_DTYPE_BF16) return mfma_bf16(a, b, c);
-  typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
                                                 0);
 }
 
-// Two f32 as 16-bit numbers, to nearest even.
-template <int DT>
+// Two f32 as f16, to nearest even.
 __device__ __forceinline__ uint32_t pack_of(float lo, float hi) {
-  if constexpr (DT == TQ_DTYPE_BF16) {
-    const bf16x2_t t = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
-    return __builtin_bit_cast(uint32_t, t);
-  } else {
-    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-    const f16x2_t t = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
-    return __builtin_bit_cast(uint32_t, t);
-  }
+  const f16x2_t t = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+  return __builtin_bit_cast(uint32_t, t);
 }
 
 // Eight codes as f32: one word of 4-bit codes or two of 8-bit ones.
@@ -86,19 +85,13 @@ __device__ __forceinline__ void codes_f32(const uint32_t* w, float (&f)[8]) {
   }
 }
 
-// Whether every value scale * code + bias rounds to a finite number of the type.
+// Whether a group's values scale * code + bias go in as f16: finite numbers of it, and its spacing near zero (2^-24)
+// no more than bf16's own at the group's largest.
 template <int DT, int BITS>
-__device__ __forceinline__ bool in_range(float2 sb) {
-  const float most = DT == TQ_DTYPE_F16 ? 65504.f : 0x1.fep127f;
-  return fabsf(sb.y) + static_cast<float>((1 << BITS) - 1) * fabsf(sb.x) <= most;  // false for NaN
-}
-
-// A value cut to the type's range; NaN and infinite pairs give zeros (the flagged way adds them).
-template <int DT>
-__device__ __forceinline__ float cut(float2 sb, float code) {
-  const float most = DT == TQ_DTYPE_F16 ? 65504.f : 0x1.fep127f;
-  if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY)) return 0.f;
-  return fminf(fmaxf(__builtin_fmaf(sb.x, code, sb.y), -most), most);
+__device__ __forceinline__ bool fits_f16(float2 sb) {
+  const float most = fabsf(sb.y) + static_cast<float>((1 << BITS) - 1) * fabsf(sb.x);
+  if (DT == TQ_DTYPE_BF16 && most < 0x1p-15f) return most == 0.f;
+  return most <= 65504.f;  // false for NaN
 }
 
 template <int DT, int KB, int VB, int KS, int CT, bool MASK>
@@ -107,7 +100,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
   constexpr int RT = S::RT;
   __shared__ __attribute__((aligned(16))) uint16_t k_lds[2][S::KBUF];
   __shared__ __attribute__((aligned(16))) uint16_t v_lds[2][S::VBUF];
-  __shared__ uint32_t bad_lds[3][2];  // tokens whose values are not finite, of three steps
+  __shared__ __attribute__((aligned(16))) uint32_t odd_lds[3][4];  // three steps' tokens whose keys, and values, f16 lacks
   __shared__ int range_lds[2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -150,6 +143,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 
   // this lane's query rows, as columns of C
   u32x4_t qop[RT][KS];
+  float unit[RT];  // scores are this times the products
   int lim[RT];
   int64_t mask_at[RT];
 #pragma unroll
@@ -158,17 +152,36 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
     const int l = row / p.R, r = row % p.R;
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb + (static_cast<int64_t>(h) * p.R + r) * p.q_sh +
                         static_cast<int64_t>(l) * p.q_sl;
+    // times the power of two that takes the row's largest magnitude to [1, 2): coordinates over 2^-14 of it keep all
+    // their bits, smaller ones are off by 2^-25 of it at most.  A negative scale turns the signs, so that the largest
+    // product has the largest score.  Exponents are clamped so that both factors stay normal.
+    float big = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const uint4 u = *reinterpret_cast<const uint4*>(q + s * 32 + q4 * 8);
       qop[rt][s] = u32x4_t{u.x, u.y, u.z, u.w};
-      // a negative scale turns the queries' signs, so that the largest product has the largest score
-      if (p.scale < 0.f) qop[rt][s] ^= u32x4_t{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 two = pair16<DT>(qop[rt][s][j]);
+        big = fmaxf(big, fmaxf(fabsf(two.x), fabsf(two.y)));
+      }
     }
+    big = fmaxf(big, __shfl_xor(big, 16));
+    big = fmaxf(big, __shfl_xor(big, 32));
+    const int up = min(max(127 - static_cast<int>(__float_as_uint(big) >> 23), -113), 113);
+    const float lift =
+        __uint_as_float((p.scale < 0.f ? 0x80000000u : 0u) | (static_cast<uint32_t>(127 + up) << 23));
+    unit[rt] = fabsf(p.scale) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 two = pair16<DT>(qop[rt][s][j]);
+        qop[rt][s][j] = pack_of(two.x * lift, two.y * lift);
+      }
     lim[rt] = p.causal ? static_cast<int>(end) - p.L + l : INT32_MAX;
     mask_at[rt] = MASK ? b * p.mask_s[0] + h * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3] : 0;
   }
-  const float scale = fabsf(p.scale);
   const bool quads = MASK && p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1;
   // the causal rule leaves a step of tokens alone when its last one is within the first row's limit
   const int lim_min = p.causal ? static_cast<int>(end) - p.L + row0 / p.R : INT32_MAX;
@@ -244,7 +257,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
     }
   };
 
-  auto decode_keys = [&](int buf) {
+  auto decode_keys = [&](int buf, int flags) {
     const uint32_t id = half_id();
     {
 #pragma unroll
@@ -252,21 +265,17 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
         const uint32_t unit = i * 256 + id;
         const uint32_t tok = unit / (KS * 4), piece = unit % (KS * 4);
         const uint32_t* w = raw + i * (KWORDS + 1);
-        const float2 sb = pair16<DT>(w[KWORDS]);
+        float2 sb = pair16<DT>(w[KWORDS]);
+        if (!fits_f16<DT, KB>(sb)) {
+          atomicOr(&odd_lds[flags][tok >> 5], 1u << (tok & 31));
+          sb = make_float2(0.f, 0.f);
+        }
         float f[8];
         codes_f32<KB>(w, f);
         u32x4_t o;
-        if (in_range<DT, KB>(sb)) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[j] = pack_of<DT>(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y));
-        } else {  // NaN stays
-          const bool nan = !(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[j] = nan ? pack_of<DT>(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y))
-                       : pack_of<DT>(cut<DT>(sb, f[2 * j]), cut<DT>(sb, f[2 * j + 1]));
-        }
+        for (int j = 0; j < 4; ++j)
+          o[j] = pack_of(__builtin_fmaf(sb.x, f[2 * j], sb.y), __builtin_fmaf(sb.x, f[2 * j + 1], sb.y));
         *reinterpret_cast<u32x4_t*>(&k_lds[buf][S::k_at(tok, piece)]) = o;
       }
     }
@@ -283,35 +292,32 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t* w = raw + (i * 4 + j) * (VWORDS + 1);
-          const float2 sb = pair16<DT>(w[VWORDS]);
-          codes_f32<VB>(w, v[j]);
-          if (in_range<DT, VB>(sb)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = __builtin_fmaf(sb.x, v[j][e], sb.y);
-          } else {
-            if (!(fabsf(sb.x) < INFINITY) || !(fabsf(sb.y) < INFINITY))
-              atomicOr(&bad_lds[flags][quad >> 3], 1u << ((quad * 4 + j) & 31));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = cut<DT>(sb, v[j][e]);
+          float2 sb = pair16<DT>(w[VWORDS]);
+          if (!fits_f16<DT, VB>(sb)) {
+            atomicOr(&odd_lds[flags][2 + (quad >> 3)], 1u << ((quad * 4 + j) & 31));
+            sb = make_float2(0.f, 0.f);
           }
+          codes_f32<VB>(w, v[j]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] = __builtin_fmaf(sb.x, v[j][e], sb.y);
         }
         // tokens 4 quad + j: 32 (quad / 8) + 8 (quad % 4) + 4 (quad / 4 % 2) + j in the order of A's k indices
         const uint32_t pos = (quad >> 3) * 32 + (quad & 3) * 8 + ((quad >> 2) & 1) * 4;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint2 two = make_uint2(pack_of<DT>(v[0][e], v[1][e]), pack_of<DT>(v[2][e], v[3][e]));
+          const uint2 two = make_uint2(pack_of(v[0][e], v[1][e]), pack_of(v[2][e], v[3][e]));
           *reinterpret_cast<uint2*>(&v_lds[buf][S::v_at(piece * 8 + e, pos >> 3) + (pos & 4)]) = two;
         }
       }
     }
   };
 
-  if (tid < 6) bad_lds[tid >> 1][tid & 1] = 0;
+  if (tid < 12) odd_lds[tid >> 2][tid & 3] = 0;
   __syncthreads();
   if (t0 < t1) {
     load(t0);
     if (keys)
-      decode_keys(0);
+      decode_keys(0, 0);
     else
       decode_values(0, 0);
     if (t0 + kTileStep < t1) load(t0 + kTileStep);
@@ -322,7 +328,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
   for (int t = t0; t < t1; t += kTileStep, buf ^= 1, flags = flags == 2 ? 0 : flags + 1) {
     const bool more = t + kTileStep < t1;
     // four tokens' bytes of a contiguous boolean mask, on their way while the scores are computed
-    uint32_t quad[RT][4];
+    uint32_t quad[RT][4] = {};
     const bool by_quads = quads && t + kTileStep <= t1;
     if (MASK && by_quads) {
 #pragma unroll
@@ -334,9 +340,14 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
     // The next tile goes into the other half of LDS, and its successor's codes on their way: the waves of the values do
     // it here, the waves of the keys at the end, so that of a SIMD's two waves one is at vector work while the other is
     // at matrix work all through the step.
-    if (tid < 2) bad_lds[flags == 0 ? 2 : flags - 1][tid] = 0;
+    if (tid < 4) odd_lds[flags == 0 ? 2 : flags - 1][tid] = 0;
     if (!keys && more) decode_values(buf ^ 1, flags == 2 ? 0 : flags + 1);
     if (!MASK && !keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
+    const u32x4_t odd_of = *reinterpret_cast<const u32x4_t*>(odd_lds[flags]);
+    auto odd_tokens = [&](int at) {  // the same for all lanes
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(odd_of[at]), hi = __builtin_amdgcn_readfirstlane(odd_of[at + 1]);
+      return static_cast<uint64_t>(hi) << 32 | lo;
+    };
     // ---- scores
     // operands a tile ahead of the products: a read of LDS takes longer than the products of the one before
     f32x4_t C[RT][4];
@@ -356,14 +367,44 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) C[rt][ti] = mfma_of<DT>(kop[ti & 1][s], qop[rt][s], C[rt][ti]);
+        for (int rt = 0; rt < RT; ++rt) C[rt][ti] = mfma_of(kop[ti & 1][s], qop[rt][s], C[rt][ti]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (MASK && by_quads) {  // the mask has arrived here, so that nothing later waits for it and the codes behind it
+    if constexpr (MASK) {  // the mask has arrived here on every way: nothing later waits for it and the codes behind it
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti) asm volatile("" : "+v"(quad[rt][ti]));
+    }
+    // ---- tokens whose keys f16 does not hold: their products in f32
+#pragma unroll 1
+    for (uint64_t odd = odd_tokens(0); __builtin_expect(odd != 0, 0); odd &= odd - 1) {
+      const int tok = __builtin_ctzll(odd);
+      if (t + tok >= t1) break;
+      const int64_t at = base + t + tok;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row0 + rt * 16 + c, p.rows - 1);
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + b * p.q_sb +
+                            (static_cast<int64_t>(h) * p.R + row % p.R) * p.q_sh + static_cast<int64_t>(row / p.R) * p.q_sl;
+        const float lift = unit[rt] == 0.f ? 0.f : p.scale / unit[rt];  // a power of two
+        float dot = 0.f;
+#pragma unroll 1
+        for (int d = q4 * (S::DK / 4); d < (q4 + 1) * (S::DK / 4); ++d) {
+          const float2 sb = pair16<DT>(static_cast<const uint32_t*>(p.k_params)[at * (S::DK >> (shift + 3)) + (d >> (shift + 3))]);
+          const uint32_t word = p.k_codes[at * (S::DK * KB / 32) + d * KB / 32];
+          const float k = __builtin_fmaf(sb.x, static_cast<float>((word >> (d * KB % 32)) & ((1u << KB) - 1u)), sb.y);
+          dot = __builtin_fmaf(pair16<DT>(q[d]).x * lift, k, dot);
+        }
+        dot += __shfl_xor(dot, 16);
+        dot += __shfl_xor(dot, 32);
+        if (q4 == tok % 16 / 4) {
+#pragma unroll
+          for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) C[rt][ti][j] = tok / 16 == ti && tok % 4 == j ? dot : C[rt][ti][j];
+        }
+      }
     }
     if (MASK && !keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
 
@@ -384,20 +425,20 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top;
-      if (plain) {
+      if (__builtin_expect(plain, 1)) {
         top = C[rt][0][0];
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
           for (int j = 0; j < 4; ++j) top = fmaxf(top, C[rt][ti][j]);
-        top *= scale;
+        top *= unit[rt];
       } else {
         top = -INFINITY;
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float y = C[rt][ti][j] * scale;
+            float y = C[rt][ti][j] * unit[rt];
             const int tok = t + ti * 16 + q4 * 4 + j;
             if (MASK && by_quads)
               y = (quad[rt][ti] >> (8 * j)) & 0xffu ? y : -FLT_MAX;
@@ -409,7 +450,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
             top = fmaxf(top, y);
           }
       }
-      if (__any(top > m[rt] + 8.f)) {
+      if (__builtin_expect(__any(top > m[rt] + 8.f), 0)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float to = fmaxf(m[rt], top);
@@ -425,11 +466,11 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
           for (int n = 0; n < CT; ++n) acc[rt][n][j] *= aj;
         }
       }
-      if (plain) {
+      if (__builtin_expect(plain, 1)) {
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) C[rt][ti][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(C[rt][ti][j], scale, -ref[rt]));
+          for (int j = 0; j < 4; ++j) C[rt][ti][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(C[rt][ti][j], unit[rt], -ref[rt]));
       } else {
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti)
@@ -441,15 +482,12 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float lo = C[rt][2 * pr + j / 2][2 * (j & 1)], hi = C[rt][2 * pr + j / 2][2 * (j & 1) + 1];
-          if constexpr (DT == TQ_DTYPE_BF16)
-            A[rt][pr][j] = pack_of<DT>(lo, hi);
-          else
-            A[rt][pr][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+          A[rt][pr][j] = pack_of(lo, hi);
         }
     }
 
     // ---- values: groups of VG operands, one ahead of the products
-    constexpr uint32_t kOnes = DT == TQ_DTYPE_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    constexpr uint32_t kOnes = 0x3c003c00u;
     constexpr int VG = KS == 8 ? 2 : CT % 4 == 0 ? 4 : 3, NGR = CT / VG;
     const u32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
     u32x4_t vop[2][VG];
@@ -467,50 +505,48 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
       __builtin_amdgcn_sched_barrier(0);
       if (at % NGR == 0) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma_of<DT>(A[rt][pr], ones, sum[rt]);
+        for (int rt = 0; rt < RT; ++rt) sum[rt] = mfma_of(A[rt][pr], ones, sum[rt]);
       }
 #pragma unroll
       for (int i = 0; i < VG; ++i)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          acc[rt][(at % NGR) * VG + i] = mfma_of<DT>(A[rt][pr], vop[at & 1][i], acc[rt][(at % NGR) * VG + i]);
+          acc[rt][(at % NGR) * VG + i] = mfma_of(A[rt][pr], vop[at & 1][i], acc[rt][(at % NGR) * VG + i]);
       __builtin_amdgcn_sched_barrier(0);
     }
 
-    // ---- tokens whose values are not finite, for the rows that weigh them
-    const uint32_t bad0 = __builtin_amdgcn_readfirstlane(bad_lds[flags][0]), bad1 = __builtin_amdgcn_readfirstlane(bad_lds[flags][1]);
-    if (bad0 | bad1) {
+    // ---- tokens with values that f16 does not hold, for the rows that weigh them
 #pragma unroll 1
-      for (int tok = 0; tok < kTileStep; ++tok) {
-        if (!(((tok < 32 ? bad0 : bad1) >> (tok & 31)) & 1u) || t + tok >= t1) continue;
-        const int64_t at = base + t + tok;
+    for (uint64_t odd = odd_tokens(2); __builtin_expect(odd != 0, 0); odd &= odd - 1) {
+      const int tok = __builtin_ctzll(odd);
+      if (t + tok >= t1) break;
+      const int64_t at = base + t + tok;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          // the rounded weight: tile tok / 16, two tokens a register
-          uint32_t two = 0;
+      for (int rt = 0; rt < RT; ++rt) {
+        // the rounded weight: tile tok / 16, two tokens a register
+        uint32_t two = 0;
 #pragma unroll
-          for (int pr = 0; pr < 2; ++pr)
+        for (int pr = 0; pr < 2; ++pr)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) two = tok / 32 == pr && tok / 16 % 2 * 2 + tok % 4 / 2 == j ? A[rt][pr][j] : two;
-          const float2 both = pair16<DT>(two);
-          const float w = tok % 2 ? both.y : both.x;
-          float wr[4];
+          for (int j = 0; j < 4; ++j) two = tok / 32 == pr && tok / 16 % 2 * 2 + tok % 4 / 2 == j ? A[rt][pr][j] : two;
+        const float2 both = pair16<TQ_DTYPE_F16>(two);
+        const float w = tok % 2 ? both.y : both.x;
+        float wr[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) wr[j] = __shfl(w, (tok % 16) / 4 * 16 + q4 * 4 + j);
+        for (int j = 0; j < 4; ++j) wr[j] = __shfl(w, (tok % 16) / 4 * 16 + q4 * 4 + j);
 #pragma unroll
-          for (int n = 0; n < CT; ++n) {
-            const int d = n * 16 + c;
-            const float2 sb = pair16<DT>(static_cast<const uint32_t*>(p.v_params)[at * (S::DV >> (shift + 3)) + (d >> (shift + 3))]);
-            if ((fabsf(sb.x) < INFINITY) && (fabsf(sb.y) < INFINITY)) continue;  // in LDS already
-            const uint32_t word = p.v_codes[at * (S::DV * VB / 32) + d * VB / 32];
-            const float v = __builtin_fmaf(sb.x, static_cast<float>((word >> (d * VB % 32)) & ((1u << VB) - 1u)), sb.y);
+        for (int n = 0; n < CT; ++n) {
+          const int d = n * 16 + c;
+          const float2 sb = pair16<DT>(static_cast<const uint32_t*>(p.v_params)[at * (S::DV >> (shift + 3)) + (d >> (shift + 3))]);
+          if (fits_f16<DT, VB>(sb)) continue;  // in LDS already
+          const uint32_t word = p.v_codes[at * (S::DV * VB / 32) + d * VB / 32];
+          const float v = __builtin_fmaf(sb.x, static_cast<float>((word >> (d * VB % 32)) & ((1u << VB) - 1u)), sb.y);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[rt][n][j] = wr[j] == 0.f ? acc[rt][n][j] : __builtin_fmaf(wr[j], v, acc[rt][n][j]);
-          }
+          for (int j = 0; j < 4; ++j) acc[rt][n][j] = wr[j] == 0.f ? acc[rt][n][j] : __builtin_fmaf(wr[j], v, acc[rt][n][j]);
         }
       }
     }
-    if (keys && more) decode_keys(buf ^ 1);
+    if (keys && more) decode_keys(buf ^ 1, flags == 2 ? 0 : flags + 1);
     if (keys && t + 2 * kTileStep < t1) load(t + 2 * kTileStep);
     __syncthreads();
   }

@@ -86,15 +86,20 @@ def attention_tolerance(q, k_params, k_bits, v, want, p, scale, dtype, group, ro
     their magnitudes, where a code may be carried as 128 + c (4 bits) or
     1024 + c (8 bits) and the group's sum taken off again.  A score's
     error dS moves a weight by 2 dS of itself at most (numerator and sum) while
-    dS is small.  ``rounded``: keys, weights and values go through the dtype
-    (many query rows); independent roundings of half a step u add up to at most
-    6 u sqrt(sum of squares).  Otherwise a weight times a scale keeps 16 bits
+    dS is small.  ``rounded``: keys, weights and values go through f16 (many
+    query rows); independent roundings of half a step u add up to at most 6 u
+    sqrt(sum of squares).  f16 ends at 2^-24: queries, brought to [1, 2), are off
+    by 2^-25 of the row's largest, weights by 2^-25 of a sum of one or more, keys
+    and values whose group's largest is 2^-15 or more by 2^-10 of that, a step u
+    once more (others, and those past 65504, meet the f32 way).  Otherwise a weight times a scale keeps 16 bits
     (two bf16 pieces, each rounded), of codes up to 143 while in flight.  The
     result is rounded once.
     """
     B, Hq, L, D = q.shape
     R = Hq // k_params.shape[1]
-    u = half_step(dtype) if rounded and dtype != torch.float32 else 0.0
+    u = 2.0 ** -11 if rounded and dtype != torch.float32 else 0.0
+    if dtype == torch.bfloat16:
+        u = 2 * u
     kp = torch.nan_to_num(k_params.double(), nan=0.0, posinf=0.0, neginf=0.0).repeat_interleave(R, 1)
     top = 128 + 15 if k_bits == 4 else 1024 + 255
     size = kp[..., 0].abs() * top + kp[..., 1].abs()                              # (B, Hq, T, groups)
@@ -102,9 +107,11 @@ def attention_tolerance(q, k_params, k_bits, v, want, p, scale, dtype, group, ro
     mag = torch.matmul(qa.sum(-1), size.transpose(-1, -2)).amax(-1) * abs(scale)  # (B, Hq, L)
     rms = torch.sqrt(torch.matmul(qa.square().sum(-1), size.square().transpose(-1, -2))).amax(-1) * abs(scale)
     dS = mag * (D / 4 + 8) * 2.0 ** -24 + 6 * u * rms + 2.0 ** -20
+    if u:
+        dS = dS + 2.0 ** -25 * q.double().abs().amax(-1) * size.sum(-1).amax(-1, keepdim=True) * group * abs(scale)
     vt = torch.nan_to_num(v.double(), nan=0.0, posinf=0.0, neginf=0.0)
     vmax = vt.abs().amax((-1, -2)).repeat_interleave(R, 1)                        # (B, Hq)
     root = p.square().sum(-1).sqrt()
     # two or three roundings of weight and value, then the pieces
-    dV = vmax[..., None] * (18 * u * root + 20 * 2.0 ** -16 * root + 2.0 ** -18)
+    dV = vmax[..., None] * (18 * u * root + 20 * 2.0 ** -16 * root + 2.0 ** -18 + (u > 0) * v.shape[2] * 2.0 ** -25)
     return half_step(dtype) * want.abs() * 1.01 + (2 * dS * vmax[..., None] + dV)[..., None] + 1e-30

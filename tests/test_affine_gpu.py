@@ -19,9 +19,9 @@ def vectors(seed, shape, dtype, spread=0.5):
     return (torch.randn(shape, generator=g) * scale).to(dtype)
 
 
-def filled(seed, B, H, T, dim, bits, group, dtype, device, cap=None, spread=0.5):
+def filled(seed, B, H, T, dim, bits, group, dtype, device, cap=None, spread=0.5, times=1.0):
     """(state viewing T tokens of capacity buffers on the device, f64 values) of quantized vectors."""
-    x = vectors(seed, (B, H, T, dim), dtype, spread)
+    x = (vectors(seed, (B, H, T, dim), torch.float32, spread) * times).to(dtype)
     words, params = A.quantize(x, bits, group)
     st = affine_state(B, H, cap or T, dim, bits, group, dtype, device)
     st.codes.view(torch.int32)[:, :, :T] = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32).to(device)
@@ -247,6 +247,33 @@ def test_masked_tokens_may_hold_nan(device, dtype, L, D):
     vs.params[:, :, (~keep).nonzero().flatten().to(device)] = math.nan
     out = attention_affine(q.to(device), ks, vs, group, 0.1)
     assert torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("L", [1, 5, 50])
+@pytest.mark.parametrize("D,group", [(128, 64), (64, 32), (256, 128)])
+@pytest.mark.parametrize("dtype,key,value", [("bf16", 1e6, 1e7), ("bf16", 1e-7, 1e-6), ("bf16", 2.0 ** -16, 2.0 ** -16),
+                                             ("bf16", 1e20, 1e30), ("bf16", 1e-20, 1e-30), ("f16", 2000.0, 2000.0),
+                                             ("f16", 2.0 ** -10, 2.0 ** -12)])
+def test_sizes_of_keys_and_values(device, dtype, key, value, D, group, L):
+    """Keys and values far from one, some tokens' alone and all of them: sixteen bits on the way to the products do not
+    show in what comes out."""
+    dt, B, Hq, Hkv, T = DTYPES[dtype], 1, 8, 2, 210
+    ks, k64 = filled(26, B, Hkv, T, D, 4, group, dt, device, times=key)
+    vs, v64 = filled(27, B, Hkv, T, D, 4, group, dt, device, times=value)
+    q = (vectors(28, (B, Hq, L, D), torch.float32, 0.0) / key).to(dt)
+    check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, 4, causal=True)
+    check(device, q, ks, vs, k64, v64, group, -1 / math.sqrt(D), dt, 4, mask=mask_of("bool", B, Hq, L, T))
+    # a few tokens of another size among ordinary ones
+    k1, k164 = filled(26, B, Hkv, T, D, 4, group, dt, device)
+    v1, v164 = filled(27, B, Hkv, T, D, 4, group, dt, device)
+    for i in (0, 63, 64, 100, 209):
+        for st, other, x, y in ((k1, ks, k164, k64), (v1, vs, v164, v64)):
+            st.codes.view(torch.int32)[:, :, i] = other.codes.view(torch.int32)[:, :, i]
+            st.params[:, :, i] = other.params[:, :, i]
+            x[:, :, i] = y[:, :, i]
+    q = vectors(28, (B, Hq, L, D), dt, 0.0)
+    check(device, q, ks, v1, k64, v164, group, 0.0, dt, 4)
+    check(device, q, k1, v1, k164, v164, group, 1 / math.sqrt(D) / max(key, 1.0), dt, 4)
 
 
 def test_many_splits_equal_few(device):
