@@ -318,9 +318,17 @@ RowsChoice rows_choice(int64_t rows, int k_dim, int v_dim, int group, int mask_k
   return r;
 }
 
-// The many-rows kernel takes what the few-rows kernel does at its head dims, for more than one block of 16 rows.
-bool tile_kernel(int64_t rows, int k_dim, int v_dim) {
-  return rows > 16 && tile_rows(k_dim, v_dim) > 0;
+// The many-rows kernel takes what the few-rows kernel does at its head dims, where it is the faster of the two: a block
+// of its rows costs what `worth` blocks of 16 cost there, whether it is full or not, and about 128 Ki tokens of those
+// pass while its first step and its join are on their way.  Microseconds, few rows / many rows: head dim 128, 64 heads
+// of 4096 tokens, 32 rows 26 / 58, 64 rows 38 / 57, 128 rows 72 / 62; 8 heads, 128 rows 21 / 27; 64: 64 rows 22 / 47,
+// 128 rows 41 / 50 and with a mask 125 / 95; 256: 32 rows 58 / 78, 48 rows 90 / 79; 96: 32 rows 47 / 54, 48 rows 70 / 54.
+bool tile_kernel(int64_t rows, int k_dim, int v_dim, int64_t heads, int64_t max_tokens, int mask_kind) {
+  const int block = tile_rows(k_dim, v_dim);
+  if (block == 0) return false;
+  const int worth = k_dim == 64 ? (mask_kind == TQ_MASK_NONE ? 9 : 5) : k_dim == 128 ? 5 : 2;
+  const int64_t more = (rows + 15) / 16 - (rows + block - 1) / block * worth;
+  return heads * max_tokens * more > 128 << 10;
 }
 
 constexpr int64_t kTileTarget = 256;  // workgroups at once: its eight waves fill a CU
@@ -425,7 +433,7 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
 
   const bool by_rows = rows_kernel(q_dtype, k_dim, v_dim, k_bits, v_bits, max_tokens);
   const RowsChoice rc = rows_choice(rows64, k_dim, v_dim, group, mask_kind);
-  const bool by_tile = by_rows && tile_kernel(rows64, k_dim, v_dim);
+  const bool by_tile = by_rows && tile_kernel(rows64, k_dim, v_dim, static_cast<int64_t>(B) * Hkv, max_tokens, mask_kind);
   const int block_rows = by_tile ? tile_rows(k_dim, v_dim) : by_rows ? rc.rows : kVecRows;
   const int64_t blocks1 = static_cast<int64_t>(B) * Hkv * ((rows64 + block_rows - 1) / block_rows);
   const bool ragged = seq_lens || seq_starts;
