@@ -19,7 +19,8 @@ __device__ __forceinline__ float code_of(const uint32_t* row, int d) {
 // S = scale * sum_g (s_g (q . c)_g + b_g sum(q)_g), an online softmax per row, O = sum p (s c + b): all in f32.
 // Wave = a quarter of the 32-coordinate blocks and lane = token for the scores, wave = row for the softmax,
 // thread = coordinate for the values.  Bound by its vector instructions, about rows * (Dk + Dv) multiply-adds a
-// token; it serves the dims that the matrix-core kernels do not take.
+// token, and by their latency at few waves; it serves f32 and the dims that the matrix-core kernels do not take (16
+// heads of 32,724 tokens, d = 128, 8 bits: 132 us, 1.3 TB/s).
 template <int DT, int KB, int VB>
 __global__ __launch_bounds__(256) void affine_vector_kernel(const AffineAttnParams p) {
   __shared__ float qs[kVecRows][kMaxDim];
@@ -230,7 +231,9 @@ __global__ __launch_bounds__(256) void affine_merge_flat_kernel(const AffineAttn
 template <int DT>
 void launch_merge(const AffineAttnParams& p, int64_t rows, hipStream_t st) {
   const int64_t quads = rows * (p.v_dim / 4);
-  // a row a workgroup hides the splits' latency where there are many of them and few rows
+  // Few splits of many rows stream through one thread for four coordinates (16,384 rows of 4 splits 9 us, 500 x 64 rows
+  // of d = 64 6 us; a workgroup a row 19 and 31); a workgroup a row hides the splits' latency where there are many of
+  // them and few rows (32 rows of 32 splits 6 us; 16).
   if (p.splits <= 16 && quads >= 65536 && quads <= INT32_MAX)
     affine_merge_flat_kernel<DT><<<static_cast<unsigned>((quads + 255) / 256), 256, 0, st>>>(
         p, static_cast<uint32_t>(p.v_dim / 4), static_cast<uint32_t>(quads));
@@ -289,10 +292,16 @@ struct Plan {
   int64_t split_tokens;
 };
 
-constexpr int64_t kVecTarget = 512;     // workgroups of the vector kernel to aim at: two a CU
-constexpr int64_t kRowsTarget = 256;    // of the few-rows kernel: eight waves, two a SIMD, on every CU
-constexpr int64_t kRaggedTarget = 768;  // where sequences end at different tokens: finer, so that CUs share the long ones
-constexpr int kRowsTokens = 512;        // tokens of one step of a workgroup's eight waves
+// Workgroups to aim at.  Vector kernel: two a CU, four where each still has 128 tokens (16 heads of 32,724 tokens in f32
+// 231 -> 132 us; 8 heads of 8192, 128 splits of 64 tokens instead of 64: 36 us against 31).
+constexpr int64_t kVecTarget = 512, kVecMore = 1024;
+// Few-rows kernel: its eight waves, two a SIMD, on every CU (8 heads of 32,768 tokens 21 us; 128: 23; 512: 31; 4 x 4
+// query rows over 4 x 131,076 tokens 149; 222; 157).
+constexpr int64_t kRowsTarget = 256;
+// Where sequences end at different tokens: finer, so that CUs share the long ones (32 sequences to 8192 tokens of
+// d = 256: 127 us; 256 workgroups 129, 1024 144, 2048 174).
+constexpr int64_t kRaggedTarget = 768;
+constexpr int kRowsTokens = 512;  // tokens of one step of a workgroup's eight waves
 
 // A split for every `unit` tokens at most, and about `target` workgroups in all.
 Plan plan_splits(int64_t blocks, int64_t max_tokens, int64_t target, int unit) {
@@ -300,6 +309,12 @@ Plan plan_splits(int64_t blocks, int64_t max_tokens, int64_t target, int unit) {
   const int64_t s = std::max<int64_t>(1, std::min(target / blocks, most));
   const int64_t per = std::max<int64_t>(1, ((max_tokens + s - 1) / s + unit - 1) / unit) * unit;
   return {static_cast<int>(std::max<int64_t>(1, (max_tokens + per - 1) / per)), per};
+}
+
+Plan vector_plan(int64_t blocks, int64_t max_tokens) {
+  const Plan two = plan_splits(blocks, max_tokens, kVecTarget, kVecTokens);
+  const Plan four = plan_splits(blocks, max_tokens, kVecMore, 2 * kVecTokens);
+  return four.splits > two.splits ? four : two;
 }
 
 int64_t rows_of(int B, int Hq, int L) { return static_cast<int64_t>(B) * Hq * L; }
@@ -352,7 +367,7 @@ Plan tile_plan(int64_t blocks, int64_t max_tokens) {
 // target / n splits, and at least one.
 int64_t most_partials(int B, int Hq, int Hkv, int L, int64_t max_tokens) {
   const int64_t rows = rows_of(B, Hq, L), most = std::max<int64_t>(1, (max_tokens + kVecTokens - 1) / kVecTokens);
-  const int64_t few = std::max(kVecTarget * kVecRows, kRaggedTarget * 16);
+  const int64_t few = std::max(kVecMore * kVecRows, kRaggedTarget * 16);
   const int64_t many = static_cast<int64_t>(Hq / Hkv) * L > 16 ? std::max(few, 2 * kTileTarget * 256) : few;
   return std::min(rows * most, many + rows);
 }
@@ -439,7 +454,7 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   const bool ragged = seq_lens || seq_starts;
   const Plan pl = by_tile ? tile_plan(blocks1, max_tokens)
                   : by_rows ? plan_splits(blocks1, max_tokens, ragged ? kRaggedTarget : kRowsTarget, kRowsTokens)
-                            : plan_splits(blocks1, max_tokens, kVecTarget, kVecTokens);
+                            : vector_plan(blocks1, max_tokens);
   AffineAttnParams p{};
   p.q = q;
   p.q_sb = q_stride_b, p.q_sh = q_stride_h, p.q_sl = q_stride_l;

