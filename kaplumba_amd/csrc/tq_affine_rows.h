@@ -53,11 +53,15 @@ struct RowsShape {
   static constexpr int NA = NGB * RPT > 16 ? NGB * RPT / 16 : 1;  // A operands a set
   static constexpr int GA = NGB / NA;                     // groups an A operand
   static constexpr int TI = 16 / (GA * RPT);              // blocks of tokens an A operand
-  static constexpr int NT = TI == 4 || DP == 64 || (DP == 128 && GS > 32 && RPT < 16) ? 4 : 2;  // 16-token tiles a step
+  // 16-token tiles a step: four where a block of tokens is one or the sums are few (d = 64, 16 rows of 64 x 32,768 tokens
+  // 66 us, by two 72); two elsewhere, for the registers (d = 256, 4 rows of 32 x 16,384 tokens 40 us, by four 108; d =
+  // 128, 4 rows of 8 x 32,768 tokens 20.1, by four 20.7)
+  static constexpr int NT = TI == 4 || DP == 64 ? 4 : 2;
   static constexpr int NU = NT / TI;                      // tiles a lane weighs
   static constexpr int STEP = 16 * NT;
   // registers that live through a step: sums, queries, codes, weights; with the temporaries, two waves a SIMD have 256
-  // each, and what needs more runs one
+  // each, and what needs more runs one (four query rows of 4 heads over 32 x 16,384 tokens, d = 256: 59 us, by eight
+  // waves 76, d = 192 55 / 76; 16 rows, d = 128, by eight 44 us, by four 57)
   static constexpr int LIVE = NS * NA * (UD + 1) * 4 + DP / 8 + NG + NT * NG * KW + NS * NT * 4 + 2 * NG +
                               NU * 4 + NS * NA * NP * NU * 2;
   static constexpr int WAVES = LIVE > 204 ? 4 : 8;
