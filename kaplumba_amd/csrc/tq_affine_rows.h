@@ -60,11 +60,11 @@ struct RowsShape {
   static constexpr int NU = NT / TI;                      // tiles a lane weighs
   static constexpr int STEP = 16 * NT;
   // registers that live through a step: sums, queries, codes, weights; with the temporaries, two waves a SIMD have 256
-  // each, and what needs more runs one (four query rows of 4 heads over 32 x 16,384 tokens, d = 256: 59 us, by eight
-  // waves 76, d = 192 55 / 76; 16 rows, d = 128, by eight 44 us, by four 57)
+  // each, and what needs more runs one (32 heads of 16,384 tokens, d = 256: 16 rows 59 us, by eight waves 76; 4 rows
+  // in groups of 32 57 us, by eight 243; d = 192, 4 rows 55 / 76; d = 128, 16 rows by eight 44 us, by four 57)
   static constexpr int LIVE = NS * NA * (UD + 1) * 4 + DP / 8 + NG + NT * NG * KW + NS * NT * 4 + 2 * NG +
                               NU * 4 + NS * NA * NP * NU * 2;
-  static constexpr int WAVES = LIVE > 204 ? 4 : 8;
+  static constexpr int WAVES = LIVE > 182 ? 4 : 8;
   static constexpr int PLANES = 4 * NG * STEP;            // floats of a wave's pairs in LDS
   static constexpr int JOIN = RPT * (DP + NG + 2);        // floats of a wave's results there, after the loop
   static constexpr int LDS = WAVES * (PLANES > JOIN ? PLANES : JOIN) * 4;

@@ -164,6 +164,23 @@ def test_many_rows(device, dtype, L, T, D, group):
           seq_lens=torch.tensor([T, max(1, T // 3)], dtype=torch.int32))
 
 
+@pytest.mark.parametrize("kb,vb", [(4, 4), (8, 4), (8, 8)])
+@pytest.mark.parametrize("D,Dv,group", [(64, 64, 32), (64, 64, 64), (96, 96, 32), (128, 128, 32), (128, 128, 64),
+                                        (128, 128, 128), (192, 128, 32), (192, 128, 64), (256, 256, 32), (256, 256, 64),
+                                        (256, 256, 128)])
+def test_layouts(device, kb, vb, D, Dv, group):
+    """Each layout's kernels: 2, 10, 40 and 180 query rows a kv head, with and without a mask; the last at enough
+    tokens for the many-rows kernel at every head dim."""
+    dt, B, Hq, Hkv = torch.bfloat16, 2, 4, 2
+    for L, T in ((1, 130), (5, 70), (20, 577), (90, 12001)):
+        ks, k64 = filled(30, B, Hkv, T, D, kb, group, dt, device)
+        vs, v64 = filled(31, B, Hkv, T, Dv, vb, group, dt, device)
+        q = vectors(32, (B, Hq, L, D), dt, 0.0)
+        check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, kb, causal=True)
+        if T < 1000:
+            check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, kb, mask=mask_of("bool", B, Hq, L, T))
+
+
 @pytest.mark.parametrize("L", [1, 3, 40])
 @pytest.mark.parametrize("dtype,D,group", [("bf16", 128, 64), ("f16", 64, 32), ("f32", 128, 64), ("bf16", 384, 64)])
 def test_ragged_and_padded(device, dtype, L, D, group):
@@ -274,6 +291,73 @@ def test_sizes_of_keys_and_values(device, dtype, key, value, D, group, L):
     q = vectors(28, (B, Hq, L, D), dt, 0.0)
     check(device, q, ks, v1, k64, v164, group, 0.0, dt, 4)
     check(device, q, k1, v1, k164, v164, group, 1 / math.sqrt(D) / max(key, 1.0), dt, 4)
+
+
+# 512 query rows a kv head over 2999 tokens: past what the few-rows kernel takes at every head dim
+MANY = [("bf16", 128, 128, 64), ("f16", 64, 64, 32), ("bf16", 96, 96, 32), ("f16", 192, 128, 64), ("bf16", 256, 256, 128)]
+
+
+def many(seed, dtype, D, Dv, group, device, kb=4, vb=4, key=1.0, value=1.0):
+    dt, B, Hq, Hkv, L, T = DTYPES[dtype], 2, 8, 2, 128, 2999
+    ks, k64 = filled(seed, B, Hkv, T, D, kb, group, dt, device, cap=3001, times=key)
+    vs, v64 = filled(seed + 1, B, Hkv, T, Dv, vb, group, dt, device, cap=3001, times=value)
+    q = (vectors(seed + 2, (B, Hq, L, D), torch.float32, 0.0) / key).to(dt)
+    return q, ks, vs, k64, v64, 1 / math.sqrt(D), dt
+
+
+@pytest.mark.parametrize("kind", ["bool", "window", "add_f32", "add_f16", "add_bf16"])
+@pytest.mark.parametrize("dtype,D,Dv,group", MANY)
+def test_many_rows_masks(device, kind, dtype, D, Dv, group):
+    q, ks, vs, k64, v64, scale, dt = many(40, dtype, D, Dv, group, device, 8, 8)
+    m = mask_of(kind, 2, 8, 128, 2999)
+    got = check(device, q, ks, vs, k64, v64, group, scale, dt, 8, mask=m)
+    if kind.startswith("add"):
+        assert (got[0, 0, 0] == 0).all()
+    check(device, q, ks, vs, k64, v64, group, scale, dt, 8, mask=m, seq_lens=torch.tensor([2999, 1777]), causal=True)
+
+
+@pytest.mark.parametrize("dtype,D,Dv,group", MANY)
+def test_many_rows_ragged_and_padded(device, dtype, D, Dv, group):
+    q, ks, vs, k64, v64, scale, dt = many(43, dtype, D, Dv, group, device, 8, 4)
+    for starts, lens in (([0, 1500], [2999, 2000]), ([2998, 0], [2999, 1]), ([7, 2999], [71, 2999])):
+        starts, lens = (torch.tensor(t, dtype=torch.int32) for t in (starts, lens))
+        for causal in (False, True):
+            check(device, q, ks, vs, k64, v64, group, scale, dt, 8, causal=causal, seq_lens=lens, seq_starts=starts)
+
+
+@pytest.mark.parametrize("dtype,D,Dv,group", MANY)
+def test_many_rows_masked_tokens_may_hold_nan(device, dtype, D, Dv, group):
+    q, ks, vs, k64, v64, scale, dt = many(46, dtype, D, Dv, group, device)
+    keep = torch.ones(2999, dtype=torch.bool)
+    keep[torch.tensor([0, 1, 70, 500, 501, 1023, 2047, 2998])] = False
+    hidden = (~keep).nonzero().flatten().to(device)
+    for st, bad in ((ks, math.nan), (vs, math.inf), (vs, math.nan)):
+        st.params[:, :, hidden] = bad
+        st.codes.view(torch.int32)[:, :, hidden] = -1
+    k64[:, :, ~keep], v64[:, :, ~keep] = 0.0, 0.0
+    for m in (keep.expand(128, 2999), torch.where(keep, 0.0, -math.inf).expand(128, 2999)):
+        got = attention_affine(q.to(device), ks, vs, group, scale, mask=m.to(device)).cpu()
+        want, _, p = A.attention(q, k64, v64, scale, mask=m)
+        tol = A.attention_tolerance(q, ks.params.cpu(), 4, v64, want, p, scale, dt, group, rounded=True)
+        assert ((got.double() - want).abs() <= tol).all()
+    ks.params[:, :, hidden] = 0.1
+    assert torch.isnan(attention_affine(q.to(device), ks, vs, group, scale)).all()
+
+
+@pytest.mark.parametrize("dtype,key,value", [("bf16", 1e6, 1e7), ("bf16", 1e-7, 1e-6), ("bf16", 2.0 ** -16, 2.0 ** -16),
+                                             ("bf16", 1e20, 1e30), ("f16", 2000.0, 2000.0)])
+@pytest.mark.parametrize("D,group", [(128, 64), (64, 32), (256, 128)])
+def test_many_rows_sizes_of_keys_and_values(device, dtype, key, value, D, group):
+    q, ks, vs, k64, v64, scale, dt = many(49, dtype, D, D, group, device, 8, 4, key, value)
+    _, k1, v1, k164, v164, _, _ = many(49, dtype, D, D, group, device, 8, 4)
+    for i in (0, 63, 64, 1000, 2998):  # a few tokens of another size among ordinary ones
+        for st, other, x, y in ((k1, ks, k164, k64), (v1, vs, v164, v64)):
+            st.codes.view(torch.int32)[:, :, i] = other.codes.view(torch.int32)[:, :, i]
+            st.params[:, :, i] = other.params[:, :, i]
+            x[:, :, i] = y[:, :, i]
+    q1 = (q.double() * key).to(dt)
+    check(device, q1, k1, v1, k164, v164, group, scale / max(key, 1.0), dt, 8, causal=True)
+    check(device, q, ks, vs, k64, v64, group, -scale, dt, 8, causal=True)
 
 
 def test_many_splits_equal_few(device):
