@@ -635,7 +635,8 @@ class QuantizedKVCache(_BaseCache):
         ops._require_device(keys, values)
         B, H, L = keys.shape[0], keys.shape[1], keys.shape[2]
         end = self.offset + L
-        if self.keys is None:
+        fresh = self.keys is None
+        if fresh:
             for t, what in ((keys, "key"), (values, "value")):
                 _check_dim(t.shape[-1], self.group_size, what)
             cap = (end + self.step - 1) // self.step * self.step
@@ -644,7 +645,12 @@ class QuantizedKVCache(_BaseCache):
             if self.keys.codes.shape[:2] != (B, H):
                 raise ValueError(f"batch/heads {(B, H)} differ from the cache's {tuple(self.keys.codes.shape[:2])}")
             self.keys, self.values = self._grow(self.keys, end), self._grow(self.values, end)
-        append_affine_kv(keys, values, self.keys, self.values, self.offset, self.group_size)
+        try:
+            append_affine_kv(keys, values, self.keys, self.values, self.offset, self.group_size)
+        except Exception:
+            if fresh:  # a refused first append leaves the cache as it was
+                self.keys, self.values = None, None
+            raise
         self.offset = end
         ks, vs = self.state
         return (_QuantizedStateProxy(ks, end, H, keys.shape[-1], B),

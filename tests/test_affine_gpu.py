@@ -460,6 +460,26 @@ def test_cache_through_a_layer(device):
     assert cache.nbytes == 252 * B * H * (D + D // 2 + 2 * (D // 64) * 4)
 
 
+def test_refused_first_append_leaves_the_cache_empty(device):
+    cache = K.QuantizedKVCache(group_size=64, bits=4)
+    k = vectors(60, (1, 2, 5, 128), torch.bfloat16).to(device)
+    for v in (k.half(), k[:, :, :4], k[:, :1]):
+        with pytest.raises(ValueError):
+            cache.update_and_fetch(k, v)
+        assert cache.empty() and cache.offset == 0 and cache.state == []
+    other = k[..., :64].half()
+    cache.update_and_fetch(other, other)
+    assert cache.offset == 5
+    with pytest.raises(ValueError):
+        cache.update_and_fetch(k, k)
+    assert cache.offset == 5
+    cache.update_and_fetch(other, other)
+    want = A.values(*A.quantize(other.cpu(), 4, 64), 4, 64)
+    back = cache.dequantize(dtype=torch.float32)[0]
+    assert back.shape == (1, 2, 10, 64)
+    assert torch.allclose(back[:, :, 5:].cpu().double(), want, rtol=2.0 ** -23, atol=0)
+
+
 def test_cache_files(device, tmp_path):
     q, k, v = (vectors(s, (1, h, 33, 64), torch.float16).to(device) for s, h in ((80, 4), (81, 2), (82, 2)))
     plain = K.KVCache()
