@@ -601,10 +601,14 @@ int launch_rows_of(const AffineAttnParams& p, hipStream_t st) {
 template <int DT, int KB, int VB, int DP, int GS, bool FULL>
 int launch_rows_at(const AffineAttnParams& p, int rpt, hipStream_t st) {
   constexpr int kLarge = rows_large(DP, GS);
-  if constexpr (FULL) {
-    if (rpt == 4) return launch_rows_of<DT, KB, VB, DP, GS, 4, true, false>(p, st);
-  } else {
+  if constexpr (!FULL) {
+    if constexpr (GS <= 64) {
+      if (p.mask_kind != TQ_MASK_NONE && rpt == 4) return launch_rows_of<DT, KB, VB, DP, GS, 4, false, true>(p, st);
+    }
     if (p.mask_kind != TQ_MASK_NONE) return launch_rows_of<DT, KB, VB, DP, GS, kLarge, false, true>(p, st);
+  }
+  if constexpr (GS <= 64) {
+    if (rpt == 4) return launch_rows_of<DT, KB, VB, DP, GS, 4, FULL, false>(p, st);
   }
   return launch_rows_of<DT, KB, VB, DP, GS, kLarge, FULL, false>(p, st);
 }
