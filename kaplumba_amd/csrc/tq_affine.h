@@ -9,6 +9,14 @@
 
 namespace tq {
 
+// The tokens that rows of the array mask see: the first and one past the last kept one of a row's tokens (those of its
+// sequence, and within its limit under the causal rule), or all of them where it keeps none (such a row weighs them
+// alike).  Rows are told apart by the axes the mask has, and by b and l where windows or the causal rule differ.
+struct MaskRows {
+  int2* range;            // [nb, ng, nr, nl]
+  int nb, ng, nr, nl;
+};
+
 struct AffineAttnParams {
   const void* q;
   int64_t q_sb, q_sh, q_sl;
@@ -21,6 +29,7 @@ struct AffineAttnParams {
   const void* mask;
   int64_t mask_s[5];
   int mask_kind;
+  MaskRows keep;          // no ranges: every token of a sequence is looked at
   int causal;
   int64_t capacity, max_tokens;
   int B, Hkv, R, L;       // R query heads a kv head
@@ -47,14 +56,6 @@ int launch_rows_k4v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, 
 int launch_rows_k8v4(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
 int launch_rows_k8v8(const AffineAttnParams& p, const RowsChoice& r, int dtype, hipStream_t st);
 
-// The tokens that rows of the array mask see: the first and one past the last kept one of a row's tokens (those of its
-// sequence, and within its limit under the causal rule), or all of them where it keeps none (such a row weighs them
-// alike).  Rows are told apart by the axes the mask has, and by b and l where windows or the causal rule differ.
-struct MaskRows {
-  int2* range;         // [nb, ng, nr, nl]
-  int nb, ng, nr, nl;
-};
-
 // The many-rows kernel (tq_affine_tile.h): 32 ks key and 16 ct value coordinates; rows a workgroup takes, 0 where no
 // instantiation has these dims.
 constexpr int tile_rows(int k_dim, int v_dim) {
@@ -62,9 +63,9 @@ constexpr int tile_rows(int k_dim, int v_dim) {
          : (k_dim == 192 && v_dim == 128) || (k_dim == 256 && v_dim == 256) ? 128 : 0;
 }
 
-int launch_tile_k4v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
-int launch_tile_k8v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
-int launch_tile_k8v8(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st);
+int launch_tile_k4v4(const AffineAttnParams& p, int dtype, hipStream_t st);
+int launch_tile_k8v4(const AffineAttnParams& p, int dtype, hipStream_t st);
+int launch_tile_k8v8(const AffineAttnParams& p, int dtype, hipStream_t st);
 
 // Tokens [start, end) of sequence b, as the device arrays say, within the cache.
 __device__ __forceinline__ void affine_range(const AffineAttnParams& p, int b, int64_t& start, int64_t& end) {

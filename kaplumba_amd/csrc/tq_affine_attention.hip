@@ -241,48 +241,73 @@ void launch_merge(const AffineAttnParams& p, int64_t rows, hipStream_t st) {
     affine_merge_kernel<DT><<<static_cast<unsigned>(rows), 256, 0, st>>>(p);
 }
 
-// One workgroup a row of MaskRows.
-__global__ __launch_bounds__(256) void affine_mask_range_kernel(const AffineAttnParams p, const MaskRows rows) {
+// One workgroup a row of MaskRows: from the front to the first kept token and from the back to the last, in pieces of
+// 16 bytes a thread where the row is contiguous bytes, four single elements otherwise.  Bound by the loads' latency, a
+// round of them a step: 16 KiB of bytes in one of 1024 threads, which few rows have (many: 256).
+__global__ __launch_bounds__(1024) void affine_mask_range_kernel(const AffineAttnParams p) {
   __shared__ int lo_s, hi_s;
+  const int tid = threadIdx.x, threads = blockDim.x;
   int at = blockIdx.x;
-  const int l = at % rows.nl;
-  at /= rows.nl;
-  const int r = at % rows.nr;
-  at /= rows.nr;
-  const int g = at % rows.ng, b = at / rows.ng;
-  int64_t start, end;
-  affine_range(p, b, start, end);
-  const int64_t seen = p.causal ? max(start, min(end, end - p.L + l + 1)) : end;
-  if (threadIdx.x == 0) lo_s = INT32_MAX, hi_s = 0;
+  const int l = at % p.keep.nl;
+  at /= p.keep.nl;
+  const int r = at % p.keep.nr;
+  at /= p.keep.nr;
+  const int g = at % p.keep.ng, b = at / p.keep.ng;
+  int64_t start64, end64;
+  affine_range(p, b, start64, end64);
+  const int start = static_cast<int>(start64), end = static_cast<int>(end64);
+  const int seen = p.causal ? static_cast<int>(max(start64, min(end64, end64 - p.L + l + 1))) : end;
+  if (tid == 0) lo_s = INT32_MAX, hi_s = 0;
   __syncthreads();
   const int64_t from = b * p.mask_s[0] + g * p.mask_s[1] + r * p.mask_s[2] + l * p.mask_s[3];
-  int lo = INT32_MAX, hi = 0;
-  auto see = [&](int64_t t, bool kept) {
-    if (kept) lo = min(lo, static_cast<int>(t)), hi = max(hi, static_cast<int>(t) + 1);
-  };
   // a NaN counts as kept
-  auto kept = [&](int64_t t) {
+  auto kept = [&](int t) {
     return !(affine_mask(p, from + t * p.mask_s[4], 0.f) <= (p.mask_kind == TQ_MASK_BOOL ? -FLT_MAX : -INFINITY));
   };
-  int64_t t0 = start;
-  if (p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1) {  // eight bytes a thread where the row is contiguous
-    const uint8_t* m = static_cast<const uint8_t*>(p.mask) + from;
-    for (; t0 + 2048 <= seen; t0 += 2048) {
-      const int64_t t = t0 + threadIdx.x * 8;
-      uint64_t w;
-      __builtin_memcpy(&w, m + t, 8);
-      if (w) {
-        see(t + (__ffsll(static_cast<unsigned long long>(w)) - 1) / 8, true);
-        see(t + (63 - __clzll(static_cast<long long>(w))) / 8, true);
+  const bool bytes = p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1;
+  const int chunk = threads * (bytes ? 16 : 4);
+  // the first and one past the last kept token of this thread's part of [t, t + chunk)
+  auto look = [&](int64_t t, int& lo, int& hi) {
+    if (bytes) {
+      const int64_t mine = t + tid * 16;
+      if (mine >= start && mine + 16 <= seen) {
+        uint64_t w[2];
+        __builtin_memcpy(w, static_cast<const uint8_t*>(p.mask) + from + mine, 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (w[i]) {
+            const int at0 = static_cast<int>(mine) + 8 * i;
+            lo = min(lo, at0 + (__ffsll(static_cast<unsigned long long>(w[i])) - 1) / 8);
+            hi = max(hi, at0 + (63 - __clzll(static_cast<long long>(w[i]))) / 8 + 1);
+          }
+      } else {
+        for (int64_t e = max(mine, start64); e < min(mine + 16, static_cast<int64_t>(seen)); ++e)
+          if (kept(static_cast<int>(e))) lo = min(lo, static_cast<int>(e)), hi = max(hi, static_cast<int>(e) + 1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t e = t + i * threads + tid;
+        if (e >= start && e < seen && kept(static_cast<int>(e)))
+          lo = min(lo, static_cast<int>(e)), hi = max(hi, static_cast<int>(e) + 1);
       }
     }
+  };
+  // from both ends at once, until each has met a kept token; the front's way alone covers every token
+  int lo = INT32_MAX, hi = 0, unused_lo = INT32_MAX, unused_hi = 0;
+  bool front = true, back = true;
+  for (int64_t t = start, e = static_cast<int64_t>(seen) - chunk; front && t < seen; t += chunk, e -= chunk) {
+    look(t, lo, unused_hi);
+    if (back) look(e, unused_lo, hi);
+    front = !__syncthreads_or(lo != INT32_MAX);
+    back = back && !__syncthreads_or(hi != 0);
+    if (!front)
+      for (; back; back = !__syncthreads_or(hi != 0)) look(e -= chunk, unused_lo, hi);
   }
-  for (int64_t t = t0 + threadIdx.x; t < seen; t += 256) see(t, kept(t));
   atomicMin(&lo_s, lo);
   atomicMax(&hi_s, hi);
   __syncthreads();
-  if (threadIdx.x == 0)
-    rows.range[blockIdx.x] = hi_s > 0 ? make_int2(lo_s, hi_s) : make_int2(static_cast<int>(start), static_cast<int>(end));
+  if (tid == 0) p.keep.range[blockIdx.x] = hi_s > 0 ? make_int2(lo_s, hi_s) : make_int2(start, end);
 }
 
 int64_t align256(int64_t n) { return (n + 255) & ~static_cast<int64_t>(255); }
@@ -348,6 +373,11 @@ bool tile_kernel(int64_t rows, int k_dim, int v_dim, int64_t heads, int64_t max_
   const int64_t more = (rows + 15) / 16 - (rows + block - 1) / block * worth;
   return heads * max_tokens * more > 128 << 10;
 }
+
+// Tokens times blocks of rows from which the few-rows kernel has the masks' ranges found first.  That costs 11 us, which
+// a mask that keeps tokens everywhere pays for nothing (2 x 8 heads of 32,768 tokens, d = 128, one query 35 -> 46 us,
+// eight 70 -> 81); a window of 512 takes 34 -> 26 and 69 -> 27 there, 805 -> 36 at 8 queries over 8 x 131,072 of 192/128.
+constexpr int64_t kRangeTokens = 512 << 10;
 
 constexpr int64_t kTileTarget = 256;  // workgroups at once: its eight waves fill a CU
 
@@ -482,19 +512,19 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
   if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned n_blocks = static_cast<unsigned>(blocks);
+  if (mask_kind != TQ_MASK_NONE && (by_tile || (by_rows && blocks1 * max_tokens >= kRangeTokens))) {
+    p.keep.range = reinterpret_cast<int2*>(static_cast<char*>(workspace) + align256(n * 8) + align256(n * v_dim * 4));
+    p.keep.nb = p.mask_s[0] || ragged ? B : 1;
+    p.keep.ng = p.mask_s[1] ? Hkv : 1;
+    p.keep.nr = p.mask_s[2] ? p.R : 1;
+    p.keep.nl = p.mask_s[3] || causal ? L : 1;
+    const unsigned mask_rows = static_cast<unsigned>(p.keep.nb * p.keep.ng * p.keep.nr * p.keep.nl);
+    affine_mask_range_kernel<<<mask_rows, mask_rows <= 256 ? 1024 : 256, 0, st>>>(p);
+  }
   if (by_tile) {
-    MaskRows mr{};
-    if (mask_kind != TQ_MASK_NONE) {
-      mr.range = reinterpret_cast<int2*>(static_cast<char*>(workspace) + align256(n * 8) + align256(n * v_dim * 4));
-      mr.nb = p.mask_s[0] || ragged ? B : 1;
-      mr.ng = p.mask_s[1] ? Hkv : 1;
-      mr.nr = p.mask_s[2] ? p.R : 1;
-      mr.nl = p.mask_s[3] || causal ? L : 1;
-      affine_mask_range_kernel<<<mr.nb * mr.ng * mr.nr * mr.nl, 256, 0, st>>>(p, mr);
-    }
-    const int rc_launch = k_bits == 4   ? launch_tile_k4v4(p, mr, q_dtype, st)
-                          : v_bits == 4 ? launch_tile_k8v4(p, mr, q_dtype, st)
-                                        : launch_tile_k8v8(p, mr, q_dtype, st);
+    const int rc_launch = k_bits == 4   ? launch_tile_k4v4(p, q_dtype, st)
+                          : v_bits == 4 ? launch_tile_k8v4(p, q_dtype, st)
+                                        : launch_tile_k8v8(p, q_dtype, st);
     if (rc_launch != TQ_OK || pl.splits == 1) return rc_launch;
   } else if (by_rows) {
     const int rc_launch = k_bits == 4   ? launch_rows_k4v4(p, rc, q_dtype, st)

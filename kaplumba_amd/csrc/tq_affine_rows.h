@@ -182,9 +182,20 @@ __global__ __launch_bounds__((64 * RowsShape<KB, VB, DP, GS, RPT>::WAVES)) void 
   const uint32_t value_mask = held_scalar(0x000f000fu), value_with = held_vector(0x43004300u);
   int64_t start64, end64;
   affine_range(p, b, start64, end64);
-  const int start = static_cast<int>(start64), end = static_cast<int>(end64);
-  const int s0 = static_cast<int>(min(start64 + split * p.split_tokens, end64));
-  const int s1 = static_cast<int>(min(end64, s0 + p.split_tokens));
+  const int end = static_cast<int>(end64);
+  int s0 = static_cast<int>(min(start64 + split * p.split_tokens, end64));
+  int s1 = static_cast<int>(min(end64, s0 + p.split_tokens));
+  if (MASK && p.keep.range) {  // a split of the tokens that any of these rows sees
+    const int64_t at = ((static_cast<int64_t>(p.keep.nb > 1 ? b : 0) * p.keep.ng + (p.keep.ng > 1 ? h : 0)) * p.keep.nr +
+                        (p.keep.nr > 1 ? q_r : 0)) * p.keep.nl + (p.keep.nl > 1 ? q_l : 0);
+    int2 t = p.keep.range[at];
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) t = make_int2(min(t.x, __shfl_xor(t.x, m)), max(t.y, __shfl_xor(t.y, m)));
+    const int first = __builtin_amdgcn_readfirstlane(t.x), stop = __builtin_amdgcn_readfirstlane(t.y);
+    const int part = (stop - first + p.splits - 1) / p.splits;
+    s0 = first + static_cast<int>(min(static_cast<int64_t>(split) * part, static_cast<int64_t>(stop - first)));
+    s1 = min(stop, s0 + part);
+  }
   const int lim = p.causal ? end - p.L + q_l : INT32_MAX;
   const int lim_min = p.causal ? end - p.L + row0 / p.R : INT32_MAX;
   // this wave's part of the slab, whole steps

@@ -95,7 +95,7 @@ __device__ __forceinline__ bool fits_f16(float2 sb) {
 }
 
 template <int DT, int KB, int VB, int KS, int CT, bool MASK>
-__global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const AffineAttnParams p, const MaskRows mrows) {
+__global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const AffineAttnParams p) {
   using S = TileShape<KS, CT>;
   constexpr int RT = S::RT;
   __shared__ __attribute__((aligned(16))) uint16_t k_lds[2][S::KBUF];
@@ -124,9 +124,9 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
     for (int i = tid; i < S::ROWS; i += 64 * kTileWaves) {
       const int row = min(block_row0 + i, p.rows - 1);
       const int l = row / p.R, r = row % p.R;
-      const int64_t at = ((static_cast<int64_t>(mrows.nb > 1 ? b : 0) * mrows.ng + (mrows.ng > 1 ? h : 0)) * mrows.nr +
-                          (mrows.nr > 1 ? r : 0)) * mrows.nl + (mrows.nl > 1 ? l : 0);
-      const int2 t = mrows.range[at];
+      const int64_t at = ((static_cast<int64_t>(p.keep.nb > 1 ? b : 0) * p.keep.ng + (p.keep.ng > 1 ? h : 0)) * p.keep.nr +
+                          (p.keep.nr > 1 ? r : 0)) * p.keep.nl + (p.keep.nl > 1 ? l : 0);
+      const int2 t = p.keep.range[at];
       lo = min(lo, t.x), hi = max(hi, t.y);
     }
     atomicMin(&range_lds[0], lo);
@@ -576,26 +576,26 @@ __global__ __launch_bounds__(64 * kTileWaves) void affine_tile_kernel(const Affi
 }
 
 template <int DT, int KB, int VB, int KS, int CT>
-int launch_tile_at(const AffineAttnParams& p, const MaskRows& m, hipStream_t st) {
+int launch_tile_at(const AffineAttnParams& p, hipStream_t st) {
   constexpr int kRows = TileShape<KS, CT>::ROWS;
   static_assert(kRows == tile_rows(32 * KS, 16 * CT), "rows a workgroup");
   const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * ((p.rows + kRows - 1) / kRows) * p.splits;
   if (blocks > INT32_MAX / 512) return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: %lld workgroups", static_cast<long long>(blocks));
   if (p.mask_kind != TQ_MASK_NONE)
-    affine_tile_kernel<DT, KB, VB, KS, CT, true><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
+    affine_tile_kernel<DT, KB, VB, KS, CT, true><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p);
   else
-    affine_tile_kernel<DT, KB, VB, KS, CT, false><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p, m);
+    affine_tile_kernel<DT, KB, VB, KS, CT, false><<<static_cast<unsigned>(blocks), 64 * kTileWaves, 0, st>>>(p);
   return check_launch("affine_tile_kernel");
 }
 
 template <int DT, int KB, int VB>
-int launch_tile_bits(const AffineAttnParams& p, const MaskRows& m, hipStream_t st) {
+int launch_tile_bits(const AffineAttnParams& p, hipStream_t st) {
   switch (p.k_dim) {
-    case 64: return launch_tile_at<DT, KB, VB, 2, 4>(p, m, st);
-    case 96: return launch_tile_at<DT, KB, VB, 3, 6>(p, m, st);
-    case 128: return launch_tile_at<DT, KB, VB, 4, 8>(p, m, st);
-    case 192: return launch_tile_at<DT, KB, VB, 6, 8>(p, m, st);
-    case 256: return launch_tile_at<DT, KB, VB, 8, 16>(p, m, st);
+    case 64: return launch_tile_at<DT, KB, VB, 2, 4>(p, st);
+    case 96: return launch_tile_at<DT, KB, VB, 3, 6>(p, st);
+    case 128: return launch_tile_at<DT, KB, VB, 4, 8>(p, st);
+    case 192: return launch_tile_at<DT, KB, VB, 6, 8>(p, st);
+    case 256: return launch_tile_at<DT, KB, VB, 8, 16>(p, st);
     default: return fail(TQ_ERR_UNSUPPORTED, "tq_attention_affine: no tile kernel for head dims %d / %d", p.k_dim, p.v_dim);
   }
 }

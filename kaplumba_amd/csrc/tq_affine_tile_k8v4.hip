@@ -3,9 +3,9 @@
 
 namespace tq {
 
-int launch_tile_k8v4(const AffineAttnParams& p, const MaskRows& m, int dtype, hipStream_t st) {
-  return dtype == TQ_DTYPE_F16 ? launch_tile_bits<TQ_DTYPE_F16, 8, 4>(p, m, st)
-                               : launch_tile_bits<TQ_DTYPE_BF16, 8, 4>(p, m, st);
+int launch_tile_k8v4(const AffineAttnParams& p, int dtype, hipStream_t st) {
+  return dtype == TQ_DTYPE_F16 ? launch_tile_bits<TQ_DTYPE_F16, 8, 4>(p, st)
+                               : launch_tile_bits<TQ_DTYPE_BF16, 8, 4>(p, st);
 }
 
 }  // namespace tq

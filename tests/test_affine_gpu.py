@@ -360,6 +360,24 @@ def test_many_rows_sizes_of_keys_and_values(device, dtype, key, value, D, group)
     check(device, q, ks, vs, k64, v64, group, -scale, dt, 8, causal=True)
 
 
+@pytest.mark.parametrize("kind", ["bool", "window", "add_f16"])
+@pytest.mark.parametrize("dtype,L,D,group", [("bf16", 1, 128, 64), ("f16", 5, 64, 64), ("bf16", 3, 192, 32)])
+def test_masks_over_many_tokens(device, kind, dtype, L, D, group):
+    """Few rows of enough tokens that the ranges of the mask are found first."""
+    dt, B, Hq, Hkv, T = DTYPES[dtype], 2, 8, 2, 66001
+    ks, k64 = filled(52, B, Hkv, T, D, 4, group, dt, device, cap=T + 3)
+    vs, v64 = filled(53, B, Hkv, T, D, 4, group, dt, device, cap=T + 3)
+    q = vectors(54, (B, Hq, L, D), dt, 0.0)
+    m = mask_of(kind, B, Hq, L, T)
+    check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, 4, mask=m)
+    check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, 4, mask=m, causal=L > 1,
+          seq_lens=torch.tensor([T, 777]), seq_starts=torch.tensor([60001, 0]))
+    near = torch.zeros(L, T, dtype=torch.bool)  # a short window far into the cache, and a row without one
+    near[:, 50000:50070] = True
+    near[0, :] = L == 1
+    check(device, q, ks, vs, k64, v64, group, 1 / math.sqrt(D), dt, 4, mask=near)
+
+
 def test_many_splits_equal_few(device):
     """A long cache, whose tokens many workgroups share, and the same call over two halves joined by hand."""
     B, Hq, Hkv, T, D, group = 1, 8, 2, 20011, 128, 64
