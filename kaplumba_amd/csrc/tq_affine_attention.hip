@@ -264,13 +264,15 @@ __global__ __launch_bounds__(1024) void affine_mask_range_kernel(const AffineAtt
   auto kept = [&](int t) {
     return !(affine_mask(p, from + t * p.mask_s[4], 0.f) <= (p.mask_kind == TQ_MASK_BOOL ? -FLT_MAX : -INFINITY));
   };
-  const bool bytes = p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1;
+  const bool bytes = p.mask_kind == TQ_MASK_BOOL && p.mask_s[4] == 1 && seen - start >= 16;
   const int chunk = threads * (bytes ? 16 : 4);
   // the first and one past the last kept token of this thread's part of [t, t + chunk)
   auto look = [&](int64_t t, int& lo, int& hi) {
     if (bytes) {
-      const int64_t mine = t + tid * 16;
-      if (mine >= start && mine + 16 <= seen) {
+      // pieces over an end move inwards, over tokens that another thread looks at too
+      int64_t mine = t + tid * 16;
+      if (mine < seen && mine + 16 > start) {
+        mine = min(max(mine, start64), static_cast<int64_t>(seen) - 16);
         uint64_t w[2];
         __builtin_memcpy(w, static_cast<const uint8_t*>(p.mask) + from + mine, 16);
 #pragma unroll
@@ -280,9 +282,6 @@ __global__ __launch_bounds__(1024) void affine_mask_range_kernel(const AffineAtt
             lo = min(lo, at0 + (__ffsll(static_cast<unsigned long long>(w[i])) - 1) / 8);
             hi = max(hi, at0 + (63 - __clzll(static_cast<long long>(w[i]))) / 8 + 1);
           }
-      } else {
-        for (int64_t e = max(mine, start64); e < min(mine + 16, static_cast<int64_t>(seen)); ++e)
-          if (kept(static_cast<int>(e))) lo = min(lo, static_cast<int>(e)), hi = max(hi, static_cast<int>(e) + 1);
       }
     } else {
 #pragma unroll
