@@ -243,8 +243,9 @@ void launch_merge(const AffineAttnParams& p, int64_t rows, hipStream_t st) {
 
 // One workgroup a row of MaskRows: from the front to the first kept token and from the back to the last, in pieces of
 // 16 bytes a thread where the row is contiguous bytes, four single elements otherwise.  Bound by the loads' latency, a
-// round of them a step: 16 KiB of bytes in one of 1024 threads, which few rows have (many: 256).
-__global__ __launch_bounds__(1024) void affine_mask_range_kernel(const AffineAttnParams p) {
+// round of them a step: 8 KiB of bytes in one of 512 threads, which few rows have (8 us before 131,072 tokens; 256
+// threads 18, 1024 at 16,384 tokens 3 more).  Many rows have 256.
+__global__ __launch_bounds__(512) void affine_mask_range_kernel(const AffineAttnParams p) {
   __shared__ int lo_s, hi_s;
   const int tid = threadIdx.x, threads = blockDim.x;
   int at = blockIdx.x;
@@ -373,9 +374,9 @@ bool tile_kernel(int64_t rows, int k_dim, int v_dim, int64_t heads, int64_t max_
   return heads * max_tokens * more > 128 << 10;
 }
 
-// Tokens times blocks of rows from which the few-rows kernel has the masks' ranges found first.  That costs 11 us, which
-// a mask that keeps tokens everywhere pays for nothing (2 x 8 heads of 32,768 tokens, d = 128, one query 35 -> 46 us,
-// eight 70 -> 81); a window of 512 takes 34 -> 26 and 69 -> 27 there, 805 -> 36 at 8 queries over 8 x 131,072 of 192/128.
+// Tokens times blocks of rows from which the few-rows kernel has the masks' ranges found first.  That costs 8 us, which
+// a mask that keeps tokens everywhere pays for nothing (2 x 8 heads of 32,768 tokens, d = 128, one query 34 -> 42 us,
+// eight 70 -> 78); a window of 512 takes 34 -> 24 and 69 -> 25 there, 805 -> 36 at 8 queries over 8 x 131,072 of 192/128.
 constexpr int64_t kRangeTokens = 512 << 10;
 
 constexpr int64_t kTileTarget = 256;  // workgroups at once: its eight waves fill a CU
@@ -518,7 +519,7 @@ int tq_attention_affine(const void* q, int q_dtype, int B, int Hq, int Hkv, int 
     p.keep.nr = p.mask_s[2] ? p.R : 1;
     p.keep.nl = p.mask_s[3] || causal ? L : 1;
     const unsigned mask_rows = static_cast<unsigned>(p.keep.nb * p.keep.ng * p.keep.nr * p.keep.nl);
-    affine_mask_range_kernel<<<mask_rows, mask_rows <= 256 ? 1024 : 256, 0, st>>>(p);
+    affine_mask_range_kernel<<<mask_rows, mask_rows <= 256 ? 512 : 256, 0, st>>>(p);
   }
   if (by_tile) {
     const int rc_launch = k_bits == 4   ? launch_tile_k4v4(p, q_dtype, st)
